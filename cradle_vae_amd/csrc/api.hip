@@ -19,7 +19,7 @@ extern "C" {
 
 const char* cradle_last_error(void) { return g_last_error; }
 
-int cradle_abi_version(void) { return 9; }
+int cradle_abi_version(void) { return 10; }
 
 // Layout of the descriptor structs as THIS library was compiled: out[0] = sizeof, out[1..] = offsetof of every
 // field in declaration order.  Returns the number of entries (or -1: unknown struct / buffer too small).
@@ -56,6 +56,15 @@ int cradle_struct_layout(const char* name, int64_t* out, int max_entries) {
     OFF(S, rowbias_n); OFF(S, rowscale); OFF(S, rowscale_n); OFF(S, act_out); OFF(S, ld_act_out); OFF(S, residual);
     OFF(S, ld_residual); OFF(S, dact_src); OFF(S, ld_dact_src); OFF(S, C2); OFF(S, ldc2); OFF(S, extra_col);
     OFF(S, precision); OFF(S, k_valid);
+    return n;
+  }
+  if (!strcmp(name, "cradle_gated_mlp_desc")) {
+    typedef cradle_gated_mlp_desc S;
+    PUT(sizeof(S));
+    OFF(S, rows); OFF(S, width); OFF(S, hidden); OFF(S, out_width); OFF(S, dtype); OFF(S, act); OFF(S, x); OFF(S, ld_x);
+    OFF(S, w_in); OFF(S, ld_w_in); OFF(S, w_out); OFF(S, ld_w_out); OFF(S, b_in); OFF(S, b_out); OFF(S, residual);
+    OFF(S, ld_residual); OFF(S, y); OFF(S, ld_y); OFF(S, saved_gu); OFF(S, saved_h); OFF(S, dy); OFF(S, ld_dy); OFF(S, dx);
+    OFF(S, ld_dx); OFF(S, dw_in); OFF(S, dw_out); OFF(S, db_in); OFF(S, db_out); OFF(S, workspace); OFF(S, workspace_bytes);
     return n;
   }
   if (!strcmp(name, "cradle_step_desc")) {

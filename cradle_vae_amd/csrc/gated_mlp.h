@@ -1,0 +1,553 @@
+// The gated feed-forward block and its backward pass:
+//   [g | u] = x W_in^T + b_in,   h = act(g) * u,   y = h W_out^T + b_out (+ residual)
+//   dh = dy W_out,  dg = dh u act'(g),  du = dh act(g)
+//   dx = [dg | du] W_in,  dW_in = [dg | du]^T x,  dW_out = dy^T h,  db_in / db_out: column sums of [dg | du] / dy
+// Two products forward (x W_in^T with both projections, the activation and the gating in its epilogue), four backward (the
+// first with the whole elementwise backward in its epilogue); mm16.h has the tile product and what bounds it.
+//
+// Numbers: bf16 / fp16 tensors multiply as they are; fp32 tensors as three bf16 planes (six products, fp32's accuracy at
+// 2.6x the rate of the fp32 matrix instruction).  Sums, pre-activations and biases are fp32.  h and [dg | du] are inputs of a
+// matrix product and so are rounded once to the operand's type: an error of the size of the result's own last rounding.
+// The saved pre-activations stay fp32 (rounded to bf16 they would put two more roundings into every gradient).
+// A handful of rows (inference of single cells) take kernels that read the weights once, coalesced, with fp32 arithmetic.
+#pragma once
+#include "mm16.h"
+
+namespace cradle {
+namespace gated {
+
+using namespace mm16;
+
+enum Act { SILU = 0, GELU = 1 };
+
+// act(g) and act'(g).  silu: g s, s = 1 / (1 + exp(-g)); gelu: g Phi(g), Phi through erf.
+__device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
+  if (act == SILU) {
+    const float s = 1.f / (1.f + expf(-g));
+    // (g s with s = 0 and g = -inf is 0 * inf: the limit is 0)
+    a = s == 0.f ? 0.f : g * s;
+    da = s == 0.f ? 0.f : s * (1.f + g * (1.f - s));
+    if (g == INFINITY) da = 1.f;
+  } else {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    const float pdf = 0.39894228040143268f * expf(-0.5f * g * g);
+    a = cdf == 0.f ? 0.f : g * cdf;
+    da = pdf == 0.f ? cdf : cdf + g * pdf;
+  }
+}
+__device__ __forceinline__ float act_only(int act, float g) {
+  if (act == SILU) {
+    const float s = 1.f / (1.f + expf(-g));
+    return s == 0.f ? 0.f : g * s;
+  }
+  const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+  return cdf == 0.f ? 0.f : g * cdf;
+}
+
+__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
+  if (dtype == CRADLE_F32) return static_cast<const float*>(p)[i];
+  const u16 b = static_cast<const u16*>(p)[i];
+  return dtype == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+  if (dtype == CRADLE_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<u16*>(p)[i] = dtype == CRADLE_BF16 ? bits_bf16(v) : bits_f16(v);
+}
+__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, f32x4 v, int n, bool vec) {
+  if (vec && n >= 4) {
+    if (dtype == CRADLE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    } else {
+      u16 s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = dtype == CRADLE_BF16 ? bits_bf16(v[e]) : bits_f16(v[e]);
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p) + i) = u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) store_as(p, i + e, dtype, v[e]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// packing: a tensor as operand planes with padded, zero-filled rows
+// ---------------------------------------------------------------------------------------------------------------
+struct PackJob {
+  const void* src;
+  u16* dst;
+  int64_t ld_src, plane;
+  int rows, cols, rows_dst, ld_dst;
+  int gap_at, gap;  // destination rows [gap_at, gap_at + gap) are zero, and so are those behind the source's last
+};
+struct PackJobs {
+  PackJob job[4];
+  int dtype;
+};
+
+// one thread per 8 destination elements; ELEM planes
+template <int ELEM, int NPL>
+__global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
+  const PackJob j = js.job[blockIdx.y];
+  const int per = j.ld_dst / 8;
+  const int64_t total = (int64_t)j.rows_dst * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int r = (int)(t / per), c0 = (int)(t % per) * 8;
+    const int src = r < j.gap_at ? r : r - j.gap;
+    const bool zero = (r >= j.gap_at && r < j.gap_at + j.gap) || src >= j.rows;
+    const int64_t s = (int64_t)src * j.ld_src + c0;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = !zero && c0 + e < j.cols ? load_as(j.src, s + e, js.dtype) : 0.f;
+    u16 p[8][NPL];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) split<ELEM, NPL>(v[e], p[e]);
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = p[2 * e][k] | (uint32_t)p[2 * e + 1][k] << 16;
+      *reinterpret_cast<u32x4*>(j.dst + k * j.plane + (int64_t)r * j.ld_dst + c0) = w;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// epilogues
+// ---------------------------------------------------------------------------------------------------------------
+// h = act(g) u as operand planes (columns [hidden, ld) zero), g and u saved
+template <int ELEM, int NPH>
+struct GateEpi {
+  static constexpr bool PAIR = true;
+  int act, hidden, hidden_p;  // hidden_p: hidden rounded up to 8
+  int dtype;
+  const void* bias;  // (2 hidden) or NULL
+  u16* h;
+  int64_t h_plane;
+  float* gu;  // (rows, 2 hidden_p) or NULL
+  template <class T>
+  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
+                                        int) const {
+    each_piece<T, T::TN / 2>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
+      if (m >= a.M || n >= hidden_p) return;
+      f32x4 g = quarter(acc[i][j], q), u = quarter(acc[i][j + T::TN / 2], q), h4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = n + e < hidden;
+        if (bias && in) {
+          g[e] += load_as(bias, n + e, dtype);
+          u[e] += load_as(bias, (int64_t)hidden + n + e, dtype);
+        }
+        h4[e] = in ? act_only(act, g[e]) * u[e] : 0.f;
+      }
+      store_planes<ELEM, NPH>(h + (int64_t)m * hidden_p + n, h_plane, h4);
+      if (gu) {
+        float* r = gu + (int64_t)m * 2 * hidden_p + n;
+        *reinterpret_cast<f32x4*>(r) = g;
+        *reinterpret_cast<f32x4*>(r + hidden_p) = u;
+      }
+    });
+  }
+};
+
+// sum over the 32 lanes of a half wave; lanes 31 and 63 have it
+__device__ __forceinline__ float half_wave_sum(float v) {
+  v += dpp_move<0xB1, 0xF>(0.f, v);
+  v += dpp_move<0x4E, 0xF>(0.f, v);
+  v += dpp_move<0x141, 0xF>(0.f, v);
+  v += dpp_move<0x140, 0xF>(0.f, v);
+  v += dpp_move<0x142, 0xA>(0.f, v);
+  return v;
+}
+
+// acc = dh: dg = dh u act'(g), du = dh act(g) as operand planes side by side (rows of 2 hidden_p, padding zero), and, for the
+// bias gradient, their fp32 column sums over this wave's rows
+template <int ELEM, int NPD>
+struct GateBwdEpi {
+  static constexpr bool PAIR = false;
+  int act, hidden, hidden_p;
+  const float* gu;
+  u16* d;  // (rows, 2 hidden_p)
+  int64_t d_plane;
+  float* partial;  // (tiles_m * WAVES_M, 2 hidden_p) or NULL
+  template <class T>
+  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int tm, int,
+                                        int wm) const {
+    const int li = lane & 31, lh = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + j * 32 + q * 8 + lh * 4;
+        f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          const int m = m0 + i * 32 + li;
+          if (m < a.M && n < hidden_p) {
+            const float* r = gu + (int64_t)m * 2 * hidden_p + n;
+            const f32x4 g = *reinterpret_cast<const f32x4*>(r), u = *reinterpret_cast<const f32x4*>(r + hidden_p);
+            const f32x4 dh = quarter(acc[i][j], q);
+            f32x4 dg, du;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float av, dav;
+              act_both(act, g[e], av, dav);
+              const bool in = n + e < hidden;
+              dg[e] = in ? dh[e] * u[e] * dav : 0.f;
+              du[e] = in ? dh[e] * av : 0.f;
+            }
+            u16* o = d + (int64_t)m * 2 * hidden_p + n;
+            store_planes<ELEM, NPD>(o, d_plane, dg);
+            store_planes<ELEM, NPD>(o + hidden_p, d_plane, du);
+            sg += dg;
+            su += du;
+          }
+        }
+        if (partial) {
+          float* p = partial + (int64_t)(tm * T::WAVES_M + wm) * 2 * hidden_p + n;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sg[e] = half_wave_sum(sg[e]);
+            su[e] = half_wave_sum(su[e]);
+          }
+          if (li == 31 && n < hidden_p) {
+            *reinterpret_cast<f32x4*>(p) = sg;
+            *reinterpret_cast<f32x4*>(p + hidden_p) = su;
+          }
+        }
+      }
+  }
+};
+
+// C (+ bias + residual) in the tensors' type.  Rows from gap_at on belong gap rows further up (the padding behind each half of
+// [dg | du]^T x); the padding rows are not stored.
+struct OutEpi {
+  static constexpr bool PAIR = false;
+  void* out;
+  int64_t ld;
+  int dtype;
+  const void* bias;
+  const void* res;
+  int64_t ld_res;
+  int rows, gap_at, gap;
+  int vec;  // rows of out are aligned for four elements at a time
+  __device__ __forceinline__ void put(int m, int n, int N, f32x4 v) const {
+    if (m >= gap_at) {
+      if (m < gap_at + gap) return;
+      m -= gap;
+    }
+    if (m >= rows) return;
+    const int left = N - n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) {
+        if (bias) v[e] += load_as(bias, n + e, dtype);
+        if (res) v[e] += load_as(res, (int64_t)m * ld_res + n + e, dtype);
+      }
+    store4(out, (int64_t)m * ld + n, dtype, v, left, vec);
+  }
+  template <class T>
+  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
+                                        int) const {
+    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
+      if (m < a.M && n < a.N) put(m, n, a.N, quarter(acc[i][j], q));
+    });
+  }
+};
+
+// fp32 partial sums of a product split along K: (splits, M, Np), Np = N rounded up to 4
+struct PartialEpi {
+  static constexpr bool PAIR = false;
+  float* partial;
+  int Np;
+  template <class T>
+  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
+                                        int) const {
+    float* base = partial + (int64_t)blockIdx.z * a.M * Np;
+    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
+      if (m < a.M && n < a.N) *reinterpret_cast<f32x4*>(base + (int64_t)m * Np + n) = quarter(acc[i][j], q);
+    });
+  }
+};
+
+// joins the splits in order and finishes the output
+static __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, int M, int N, int Np,
+                                                   const OutEpi epi) {
+  const int64_t per = Np / 4, total = (int64_t)M * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    f32x4 s = {0, 0, 0, 0};
+    for (int z = 0; z < splits; ++z) s += *reinterpret_cast<const f32x4*>(partial + (int64_t)z * M * Np + t * 4);
+    epi.put((int)(t / per), (int)(t % per) * 4, N, s);
+  }
+}
+
+// column sums in two passes with a fixed order.  First: blockIdx.y-th share of the rows of a (rows, cols) tensor.
+static __global__ __launch_bounds__(256) void colsum_kernel(const void* __restrict__ src, int64_t ld, int dtype, int rows, int cols,
+                                                     int rows_per, float* __restrict__ partial) {
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int r1 = min(rows, (int)(blockIdx.y + 1) * rows_per);
+  __shared__ float red[4][64];
+  float s = 0.f;
+  if (c < cols)
+    for (int r = blockIdx.y * rows_per + w; r < r1; r += 4) s += load_as(src, (int64_t)r * ld + c, dtype);
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < cols)
+    partial[(int64_t)blockIdx.y * cols + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+// Second: sums `n` partial rows of `ld` floats; columns [0, cols), of which those from gap_at on are read gap further right
+static __global__ __launch_bounds__(256) void colsum_join_kernel(const float* __restrict__ partial, int n, int ld, int cols, int gap_at,
+                                                          int gap, void* __restrict__ out, int dtype) {
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  __shared__ float red[4][64];
+  float s = 0.f;
+  if (c < cols)
+    for (int r = w; r < n; r += 4) s += partial[(int64_t)r * ld + c + (c >= gap_at ? gap : 0)];
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < cols)
+    store_as(out, c, dtype, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------
+inline int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
+inline int esize(int dtype) { return dtype == CRADLE_F32 ? 4 : 2; }
+
+constexpr int kFewRows = 4;   // rows up to which the weights' reading bounds the block (measured beside few_rows)
+constexpr int kCUs = 256;
+
+struct Plan {
+  int M, K, F, O, Fp;
+  int dtype, elem, npl;  // planes of the tensors' operands
+  int nph;               // planes of h and [dg | du]
+};
+
+inline Plan plan_of(const cradle_gated_mlp_desc* d) {
+  Plan p;
+  p.M = d->rows;
+  p.K = d->width;
+  p.F = d->hidden;
+  p.O = d->out_width;
+  p.Fp = (int)up8(p.F);
+  p.dtype = d->dtype;
+  p.elem = d->dtype == CRADLE_F16 ? F16 : BF16;
+  p.npl = d->dtype == CRADLE_F32 ? 3 : 1;
+  p.nph = p.npl;
+  return p;
+}
+
+// a 16-bit tensor whose rows can be staged as they lie in memory
+inline bool direct(const void* p, int64_t ld, int cols, int dtype) {
+  return dtype != CRADLE_F32 && cols % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0;
+}
+
+struct Bump {
+  char* base;
+  int64_t off = 0;
+  void* take(int64_t bytes) {
+    void* r = base ? base + off : nullptr;
+    off += align256(bytes);
+    return r;
+  }
+};
+
+// operand of tensor `src` (rows x cols): itself, or packed into the workspace (a job is queued)
+// with rows_dst rows, gap of them between the two halves
+inline Operand operand(const Plan& p, const void* src, int64_t ld, int rows, int cols, int rows_dst, int gap_at, int gap, Bump& ws,
+                PackJobs& js, int& n_jobs) {
+  if (direct(src, ld, cols, p.dtype) && gap == 0) return {static_cast<const u16*>(src), ld, 0, 0};
+  const int64_t ldp = up8(cols), plane = (int64_t)rows_dst * ldp;
+  u16* dst = static_cast<u16*>(ws.take(plane * p.npl * 2));
+  js.job[n_jobs++] = {src, dst, ld, plane, rows, cols, rows_dst, (int)ldp, gap_at, gap};
+  return {dst, ldp, plane, 0};
+}
+
+template <int ELEM, int NPL>
+void run_pack(const Plan& p, PackJobs& js, int n_jobs, hipStream_t s) {
+  if (!n_jobs) return;
+  js.dtype = p.dtype;
+  int64_t most = 0;
+  for (int i = 0; i < n_jobs; ++i) {
+    const int64_t t = (int64_t)js.job[i].rows_dst * (js.job[i].ld_dst / 8);
+    most = t > most ? t : most;
+  }
+  const int64_t blocks = (most + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)n_jobs);
+  hipLaunchKernelGGL((pack_kernel<ELEM, NPL>), grid, dim3(256), 0, s, js);
+}
+
+// Tiles: 256 x 256 (eight waves) when the product fills the chip with them, else 128 x 128 (four waves); three planes need
+// half the K step and, at the large size, half the columns to fit the LDS.
+template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+struct Tiles {
+  static constexpr bool ONE = NPA == 1 && NPB == 1;
+  using Large = Tile<ELEM, NPA, NPB, 256, ONE ? 256 : 128, ONE ? 64 : 32, ONE ? 2 : 4, ONE ? 4 : 2, AK, BK>;
+  using Small = Tile<ELEM, NPA, NPB, 128, 128, ONE ? 64 : 32, 2, 2, AK, BK>;
+};
+
+template <class T, class Epi>
+void launch(Args a, const Epi& epi, int cols, int splits, hipStream_t s) {
+  a.tiles_m = (a.M + T::BM - 1) / T::BM;
+  const int bn = Epi::PAIR ? T::BN / 2 : T::BN;
+  a.tiles_n = (cols + bn - 1) / bn;
+  const int k_tiles = (a.K + T::BK - 1) / T::BK;
+  a.k_tiles_per_split = (k_tiles + splits - 1) / splits;
+  a.symmetric = 0;
+  hipLaunchKernelGGL((product_kernel<T, Epi>), dim3((unsigned)(a.tiles_m * a.tiles_n), 1, (unsigned)splits), dim3(T::NT), 0, s, a, epi);
+}
+
+template <class T>
+int64_t tiles(const Args& a, int cols, bool pair) {
+  const int bn = pair ? T::BN / 2 : T::BN;
+  return (int64_t)((a.M + T::BM - 1) / T::BM) * ((cols + bn - 1) / bn);
+}
+
+// large tiles pay while they leave no CU idle for long: at least one full wave of workgroups, the last one well filled
+inline bool use_large(int64_t n) { return n >= kCUs && (n % kCUs == 0 || n % kCUs >= kCUs / 2 || n >= 4 * kCUs); }
+
+template <int ELEM, int NPA, int NPB, bool AK, bool BK, class Epi>
+void product(const Args& a, const Epi& epi, int cols, hipStream_t s) {
+  using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
+  if (use_large(tiles<typename TT::Large>(a, cols, Epi::PAIR))) launch<typename TT::Large>(a, epi, cols, 1, s);
+  else launch<typename TT::Small>(a, epi, cols, 1, s);
+}
+
+// A product whose output has too few tiles for the chip is split along K, into shares of at least eight K tiles.
+template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+int splits_of(const Args& a) {
+  using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
+  if (use_large(tiles<typename TT::Large>(a, a.N, false))) return 1;
+  const int64_t t = tiles<typename TT::Small>(a, a.N, false);
+  const int k_tiles = (a.K + TT::Small::BK - 1) / TT::Small::BK;
+  int64_t want = (2 * kCUs + t - 1) / t;
+  const int most = k_tiles / 8;
+  if (t >= kCUs) want = 1;
+  return (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+}
+
+template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+void product_out(const Args& a, const OutEpi& epi, float* partial, hipStream_t s) {
+  const int splits = splits_of<ELEM, NPA, NPB, AK, BK>(a);
+  if (splits == 1) return product<ELEM, NPA, NPB, AK, BK>(a, epi, a.N, s);
+  using Small = typename Tiles<ELEM, NPA, NPB, AK, BK>::Small;
+  const int Np = (a.N + 3) & ~3;
+  const int k_tiles = (a.K + Small::BK - 1) / Small::BK, per = (k_tiles + splits - 1) / splits;
+  const int used = (k_tiles + per - 1) / per;  // (every share has work)
+  launch<Small>(a, PartialEpi{partial, Np}, a.N, used, s);
+  const int64_t threads = (int64_t)a.M * (Np / 4), blocks = (threads + 255) / 256;
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, partial, used, a.M, a.N, Np, epi);
+}
+
+template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+int64_t partial_floats(int M, int N, int K) {
+  Args a{};
+  a.M = M, a.N = N, a.K = K;
+  const int s = splits_of<ELEM, NPA, NPB, AK, BK>(a);
+  return s == 1 ? 0 : (int64_t)s * M * ((N + 3) & ~3);
+}
+
+inline int vec_ok(const void* p, int64_t ld, int dtype) { return ld % 4 == 0 && ((uintptr_t)p & (dtype == CRADLE_F32 ? 15 : 7)) == 0; }
+constexpr int kNoGap = 0x7fffffff;
+
+inline Args args_of(const Operand& A, const Operand& B, int M, int N, int K) {
+  Args a{};
+  a.A = A, a.B = B, a.M = M, a.N = N, a.K = K;
+  return a;
+}
+
+// ---- forward: workspace = packed x, W_in, W_out | h when it is not saved | partial sums
+template <int ELEM, int NPL>
+int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
+  Bump ws{static_cast<char*>(workspace)};
+  PackJobs js{};
+  int n = 0;
+  const int gap = p.Fp - p.F;
+  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, ws, js, n);
+  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, ws, js, n);
+  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
+  const int64_t h_plane = (int64_t)p.M * p.Fp;
+  u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * p.nph * 2));
+  float* partial = static_cast<float*>(ws.take(partial_floats<ELEM, NPL, NPL, true, true>(p.M, p.O, p.Fp) * 4));
+  if (!run) return ws.off;
+  run_pack<ELEM, NPL>(p, js, n, s);
+  Args a = args_of(x, w_in, p.M, p.F, p.K);
+  a.up_row = p.Fp;
+  product<ELEM, NPL, NPL, true, true>(
+      a, GateEpi<ELEM, NPL>{d->act, p.F, p.Fp, p.dtype, d->b_in, h, h_plane, static_cast<float*>(d->saved_gu)}, p.F, s);
+  const Operand hop{h, p.Fp, h_plane, 0};
+  product_out<ELEM, NPL, NPL, true, true>(
+      args_of(hop, w_out, p.M, p.O, p.Fp),
+      OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, vec_ok(d->y, d->ld_y, p.dtype)}, partial, s);
+  return ws.off;
+}
+
+constexpr int kColsumRows = 256;  // rows per first-pass share of a column sum, more when there are more than 512 shares
+inline int colsum_rows(int rows) {
+  const int most = (rows + 511) / 512;
+  return most > kColsumRows ? most : kColsumRows;
+}
+
+// ---- backward: workspace = packed x, W_in, W_out, dy | [dg | du] | partial sums | column-sum partials
+template <int ELEM, int NPL>
+int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
+  Bump ws{static_cast<char*>(workspace)};
+  PackJobs js{};
+  int n = 0;
+  const int gap = p.Fp - p.F;
+  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, ws, js, n);
+  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, ws, js, n);
+  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
+  const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, ws, js, n);
+  const int64_t h_plane = (int64_t)p.M * p.Fp, d_plane = 2 * h_plane;
+  u16* dgu = static_cast<u16*>(ws.take(d_plane * p.nph * 2));
+  int64_t pf = partial_floats<ELEM, NPL, NPL, true, false>(p.M, p.K, 2 * p.Fp);
+  const int64_t pf1 = partial_floats<ELEM, NPL, NPL, false, false>(2 * p.Fp, p.K, p.M);
+  const int64_t pf2 = partial_floats<ELEM, NPL, NPL, false, false>(p.O, p.F, p.M);
+  pf = pf > pf1 ? pf : pf1;
+  pf = pf > pf2 ? pf : pf2;
+  float* partial = static_cast<float*>(ws.take(pf * 4));
+  const int sum_rows = (p.M + 255) / 256 * 4;  // of either tile size: 256 rows are at most four wave rows
+  float* sums = static_cast<float*>(ws.take(d->db_in ? (int64_t)sum_rows * 2 * p.Fp * 4 : 0));
+  const int per = colsum_rows(p.M), shares = (p.M + per - 1) / per;
+  float* sums_out = static_cast<float*>(ws.take(d->db_out ? (int64_t)shares * p.O * 4 : 0));
+  if (!run) return ws.off;
+  run_pack<ELEM, NPL>(p, js, n, s);
+
+  Args a = args_of(dy, w_out, p.M, p.F, p.O);
+  using TT = Tiles<ELEM, NPL, NPL, true, false>;
+  const bool large = use_large(tiles<typename TT::Large>(a, p.F, false));
+  product<ELEM, NPL, NPL, true, false>(
+      a, GateBwdEpi<ELEM, NPL>{d->act, p.F, p.Fp, static_cast<const float*>(d->saved_gu), dgu, d_plane, d->db_in ? sums : nullptr}, p.F, s);
+  if (d->db_in) {
+    const int used = large ? (p.M + 255) / 256 * TT::Large::WAVES_M : (p.M + 127) / 128 * TT::Small::WAVES_M;
+    hipLaunchKernelGGL(colsum_join_kernel, dim3((2 * p.F + 63) / 64), dim3(256), 0, s, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
+  }
+  if (d->db_out) {
+    hipLaunchKernelGGL(colsum_kernel, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.dtype, p.M, p.O, per, sums_out);
+    hipLaunchKernelGGL(colsum_join_kernel, dim3((p.O + 63) / 64), dim3(256), 0, s, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
+  }
+  const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
+  const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};
+  auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g) {
+    return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, vec_ok(q, ld, p.dtype)};
+  };
+  if (d->dx) product_out<ELEM, NPL, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0), partial, s);
+  if (d->dw_in) product_out<ELEM, NPL, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap), partial, s);
+  if (d->dw_out) product_out<ELEM, NPL, NPL, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0), partial, s);
+  return ws.off;
+}
+
+// Both passes per type, each in a source of its own (gated_mlp_{f32,bf16,f16}.hip).  run = false: only the workspace is sized.
+#define CRADLE_GATED_TYPE(NAME) \
+  int64_t forward_##NAME(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);  \
+  int64_t backward_##NAME(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+CRADLE_GATED_TYPE(f32)
+CRADLE_GATED_TYPE(bf16)
+CRADLE_GATED_TYPE(f16)
+#undef CRADLE_GATED_TYPE
+
+}  // namespace gated
+}  // namespace cradle

@@ -93,6 +93,24 @@ PROTOTYPES = {
     "cradle_obs_counts_pairs": (i32, [ctypes.c_void_p, c_float_p, i64, i32, i32, ctypes.c_void_p, c_stream]),
     "cradle_peer_median": (i32, [ctypes.c_void_p, i32, i64, i32, ctypes.c_void_p, i64, i32, ctypes.c_void_p,
                                  ctypes.c_void_p, c_stream]),
+    "cradle_layer_norm_fwd": (i32, [ctypes.c_void_p, i64, ctypes.c_void_p, ctypes.c_void_p, i32, i32, ctypes.c_float,
+                                    ctypes.c_void_p, i64, c_float_p, c_float_p, i64, i32, c_stream]),
+    "cradle_layer_norm_workspace_floats": (i64, [i64, i32]),
+    "cradle_layer_norm_bwd": (
+        i32,
+        [ctypes.c_void_p, i64, ctypes.c_void_p, i64, ctypes.c_void_p, c_float_p, c_float_p, i32, i32, ctypes.c_void_p, i64,
+         ctypes.c_void_p, ctypes.c_void_p, c_float_p, i64, i64, i32, c_stream],
+    ),
+    "cradle_gated_mlp_saved_bytes": (i64, [i32, i32, i32, ctypes.POINTER(i64)]),
+    "cradle_gated_mlp_workspace_bytes": (i64, [ctypes.c_void_p, i32]),
+    "cradle_gated_mlp_fwd": (i32, [ctypes.c_void_p, c_stream]),
+    "cradle_gated_mlp_bwd": (i32, [ctypes.c_void_p, c_stream]),
+    "cradle_orthogonalize_workspace_bytes": (i64, [i32, i32, i32]),
+    "cradle_orthogonalize": (
+        i32,
+        [ctypes.c_void_p, i64, i64, ctypes.c_void_p, i64, i64, i32, i32, i32, i32, i32, ctypes.c_float, ctypes.c_float,
+         ctypes.c_float, ctypes.c_float, ctypes.c_void_p, i64, c_stream],
+    ),
     "cradle_nb_sample_accumulate_ws": (
         i32,
         [c_float_p, i64, c_float_p, i32, c_float_p, c_float_p, c_float_p, i32, i32, i32, i32, i32, ctypes.c_uint64,
@@ -107,7 +125,7 @@ PROTOTYPES = {
 }
 
 MAX_LAYERS = 8
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 
 class MlpPtrs(ctypes.Structure):
@@ -178,6 +196,20 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class GatedMlpDesc(ctypes.Structure):
+    """struct cradle_gated_mlp_desc (include/cradle_hip.h); field order is ABI."""
+
+    _fields_ = (
+        [(k, i32) for k in ("rows", "width", "hidden", "out_width", "dtype", "act")]
+        + [("x", ctypes.c_void_p), ("ld_x", i64), ("w_in", ctypes.c_void_p), ("ld_w_in", i64), ("w_out", ctypes.c_void_p),
+           ("ld_w_out", i64), ("b_in", ctypes.c_void_p), ("b_out", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+           ("ld_residual", i64), ("y", ctypes.c_void_p), ("ld_y", i64), ("saved_gu", ctypes.c_void_p),
+           ("saved_h", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("ld_dy", i64), ("dx", ctypes.c_void_p), ("ld_dx", i64)]
+        + [(k, ctypes.c_void_p) for k in ("dw_in", "dw_out", "db_in", "db_out", "workspace")]
+        + [("workspace_bytes", i64)]
+    )
+
+
 class CradleHipError(RuntimeError):
     pass
 
@@ -204,7 +236,7 @@ def load() -> ctypes.CDLL:
         raise CradleHipError(f"{_LIB_PATH} has ABI version {lib.cradle_abi_version()}, this binding expects "
                              f"{ABI_VERSION}: rebuild it (make -C cradle_vae_amd/csrc)")
     for cname, cls in (("cradle_mlp_ptrs", MlpPtrs), ("cradle_gemm_desc", GemmDesc), ("cradle_step_desc", StepDesc),
-                       ("cradle_batch_desc", BatchDesc)):
+                       ("cradle_batch_desc", BatchDesc), ("cradle_gated_mlp_desc", GatedMlpDesc)):
         mine, theirs = struct_layout(cls), library_struct_layout(lib, cname)
         if mine != theirs:
             raise CradleHipError(f"layout of {cname} differs between include/cradle_hip.h as compiled "

@@ -5,6 +5,7 @@ the HIP kernels.  Autograd wiring lives in ``cradle_vae_amd.functional``.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -426,4 +427,267 @@ def peer_median(src: torch.Tensor, peers: torch.Tensor) -> torch.Tensor:
                                             out.data_ptr(), flags.data_ptr(), hip.stream()), "peer_median")
     if int(flags.item()) & 1:
         raise hip.CradleHipError("peer_median: a peer index lies outside the source matrix")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# normalised, gated hidden layers and the orthogonalised update (csrc/{layer_norm,gated_mlp,orthogonalize}.hip)
+# ---------------------------------------------------------------------------------------------------------------
+FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` (..., D) as a 2-D view (or copy, where no view exists) with unit column stride and rows that do not overlap."""
+    if not t.is_cuda or t.dtype not in FLOAT_TYPES:
+        raise hip.CradleHipError(f"{what}: expected an fp32 / bf16 / fp16 CUDA tensor, got {t.dtype} on {t.device} (no fallback path)")
+    if t.dim() < 1:
+        raise hip.CradleHipError(f"{what}: expected at least one axis")
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.new_empty((0, 0))
+    if r.shape[0] and r.shape[1] and (r.stride(1) != 1 or (r.shape[0] > 1 and r.stride(0) < r.shape[1])):
+        r = r.contiguous()
+    return r
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _same_place(what: str, ref: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and (t.device != ref.device or not t.is_cuda):
+            raise hip.CradleHipError(f"{what}: {name} is on {t.device}, x on {ref.device}")
+
+
+def _vector(what: str, name: str, t: Optional[torch.Tensor], n: int, dtypes) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype not in dtypes or tuple(t.shape) != (n,):
+        raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, expected ({n},) of {' or '.join(str(d) for d in dtypes)}")
+    return t.contiguous()
+
+
+def _pointer(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """Makes a tensor's device the current one around a launch: the kernel runs on that device's current stream."""
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return hip.stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
+    """Layer norm over the last axis -> (y, mean, rstd); mean and rstd (fp32, one per row) are what ``layer_norm_bwd`` reads.
+    ``x`` fp32 / bf16 / fp16, rows may be strided; ``weight`` / ``bias`` of x's type or fp32 (``cradle_layer_norm_fwd``)."""
+    x2 = _rows_of(x, "layer_norm")
+    D = x.shape[-1]
+    types = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
+    weight, bias = _vector("layer_norm", "weight", weight, D, types), _vector("layer_norm", "bias", bias, D, types)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise hip.CradleHipError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    _same_place("layer_norm", x, weight=weight, bias=bias)
+    rows = x2.shape[0]
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
+    param = weight if weight is not None else bias
+    w_type = FLOAT_TYPES[param.dtype if param is not None else x.dtype]
+    with _on(x) as s:
+        hip.check(hip.load().cradle_layer_norm_fwd(
+            x2.data_ptr(), _ld(x2), _pointer(weight), _pointer(bias), FLOAT_TYPES[x.dtype], w_type, eps, y.data_ptr(), D,
+            stats[0].data_ptr(), stats[1].data_ptr(), rows, D, s), "layer_norm_fwd")
+    return y, stats[0], stats[1]
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor, *,
+                   need_dx: bool = True, need_params: bool = True, param_dtype: Optional[torch.dtype] = None):
+    """-> (dx, dweight, dbias) of ``layer_norm``; the parameters' gradients have weight's type (``param_dtype`` without a
+    weight, default x's) and are sums over the rows in a fixed order."""
+    what = "layer_norm_bwd"
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)}, x {x.dtype} {tuple(x.shape)}")
+    x2, dy2 = _rows_of(x, what), _rows_of(dy, what)
+    rows, D = x2.shape[0], x.shape[-1]
+    types = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
+    weight = _vector(what, "weight", weight, D, types)
+    p_dtype = weight.dtype if weight is not None else (param_dtype or x.dtype)
+    if p_dtype not in types:
+        raise hip.CradleHipError(f"{what}: param_dtype {p_dtype} is neither x's type nor fp32")
+    mean, rstd = _vector(what, "mean", mean.reshape(-1), rows, (torch.float32,)), _vector(what, "rstd", rstd.reshape(-1), rows, (torch.float32,))
+    _same_place(what, x, dy=dy, weight=weight, mean=mean, rstd=rstd)
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_dx else None
+    if rows == 0:
+        z = torch.zeros((2, D), device=x.device, dtype=p_dtype) if need_params else (None, None)
+        return dx, z[0], z[1]
+    dp = torch.empty((2, D), device=x.device, dtype=p_dtype) if need_params else (None, None)
+    lib = hip.load()
+    need = lib.cradle_layer_norm_workspace_floats(rows, D) if need_params else 0
+    ws = torch.empty(need, device=x.device, dtype=torch.float32) if need else None
+    with _on(x) as s:
+        hip.check(lib.cradle_layer_norm_bwd(
+            dy2.data_ptr(), _ld(dy2), x2.data_ptr(), _ld(x2), _pointer(weight), mean.data_ptr(), rstd.data_ptr(),
+            FLOAT_TYPES[x.dtype], FLOAT_TYPES[p_dtype], _pointer(dx), D, _pointer(dp[0]), _pointer(dp[1]), _pointer(ws), need, rows,
+            D, s), what)
+    return dx, dp[0], dp[1]
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _gated_desc(what, x, w_in, w_out, act):
+    if act not in ACTIVATIONS:
+        raise hip.CradleHipError(f"{what}: act={act!r}, expected one of {sorted(ACTIVATIONS)}")
+    if w_in.dim() != 2 or w_out.dim() != 2 or w_in.shape[0] != 2 * w_out.shape[1] or w_in.shape[1] != x.shape[-1] or 0 in w_in.shape \
+            or 0 in w_out.shape:
+        raise hip.CradleHipError(f"{what}: x {tuple(x.shape)}, w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)}: expected "
+                                 "(..., width), (2 hidden, width), (out, hidden)")
+    if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
+        raise hip.CradleHipError(f"{what}: x is {x.dtype}, w_in {w_in.dtype}, w_out {w_out.dtype}")
+    _same_place(what, x, w_in=w_in, w_out=w_out)
+    x2, wi, wo = _rows_of(x, what), _rows_of(w_in, what), _rows_of(w_out, what)
+    d = hip.GatedMlpDesc()
+    d.rows, d.width, d.hidden, d.out_width = x2.shape[0], x2.shape[1], wo.shape[1], wo.shape[0]
+    d.dtype, d.act = FLOAT_TYPES[x.dtype], ACTIVATIONS[act]
+    d.x, d.ld_x, d.w_in, d.ld_w_in, d.w_out, d.ld_w_out = x2.data_ptr(), _ld(x2), wi.data_ptr(), _ld(wi), wo.data_ptr(), _ld(wo)
+    return d, (x2, wi, wo)
+
+
+def _gated_workspace(d, backward: int, device) -> torch.Tensor:
+    import ctypes
+
+    need = hip.load().cradle_gated_mlp_workspace_bytes(ctypes.byref(d), backward)
+    if need < 0:
+        hip.check(1, "gated_mlp_workspace_bytes")
+    ws = torch.empty(max(need, 16), device=device, dtype=torch.uint8)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    return ws
+
+
+def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
+              b_out: Optional[torch.Tensor] = None, *, act: str = "silu", residual: Optional[torch.Tensor] = None, save: bool = False):
+    """Gated feed-forward block: [g | u] = x w_in^T + b_in; y = (act(g) * u) w_out^T + b_out (+ residual).  ``w_in``
+    (2 hidden, width) holds the gate's rows, then the up projection's; ``act`` "silu" or "gelu" (erf); all tensors of one type, fp32 /
+    bf16 / fp16 (``cradle_gated_mlp_fwd``).  ``save``: -> (y, saved), what ``gated_mlp_bwd`` reads (the pre-activations in
+    fp32 and h); a few rows without ``save`` take the form for single cells, which reads the weights once."""
+    import ctypes
+
+    what = "gated_mlp"
+    d, keep = _gated_desc(what, x, w_in, w_out, act)
+    M, O, F = d.rows, d.out_width, d.hidden
+    b_in, b_out = _vector(what, "b_in", b_in, 2 * F, (x.dtype,)), _vector(what, "b_out", b_out, O, (x.dtype,))
+    _same_place(what, x, b_in=b_in, b_out=b_out, residual=residual)
+    d.b_in, d.b_out = _pointer(b_in), _pointer(b_out)
+    y = torch.empty((*x.shape[:-1], O), device=x.device, dtype=x.dtype)
+    d.y, d.ld_y = y.data_ptr(), O
+    if residual is not None:
+        if residual.shape != y.shape or residual.dtype != x.dtype:
+            raise hip.CradleHipError(f"{what}: residual is {residual.dtype} {tuple(residual.shape)}, expected {x.dtype} {tuple(y.shape)}")
+        r2 = _rows_of(residual, what)
+        d.residual, d.ld_residual = r2.data_ptr(), _ld(r2)
+    lib, saved = hip.load(), None
+    if save:
+        hb = ctypes.c_int64()
+        gb = lib.cradle_gated_mlp_saved_bytes(M, F, d.dtype, ctypes.byref(hb))
+        saved = (torch.empty(gb // 4, device=x.device, dtype=torch.float32), torch.empty(hb.value // 2, device=x.device, dtype=torch.int16))
+        if M:
+            d.saved_gu, d.saved_h = saved[0].data_ptr(), saved[1].data_ptr()
+    if M:
+        ws = _gated_workspace(d, 0, x.device)
+        with _on(x) as s:
+            hip.check(lib.cradle_gated_mlp_fwd(ctypes.byref(d), s), "gated_mlp_fwd")
+    return (y, saved) if save else y
+
+
+def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, saved, *, act: str = "silu",
+                  bias: bool = False, need=(True, True, True)):
+    """-> (dx, dw_in, dw_out, db_in, db_out) of ``gated_mlp``; ``need`` says which of the first three are wanted (None in the
+    place of the others), ``bias`` whether the biases' gradients are.  The residual's gradient is dy itself."""
+    import ctypes
+
+    what = "gated_mlp_bwd"
+    d, keep = _gated_desc(what, x, w_in, w_out, act)
+    M, K, O, F = d.rows, d.width, d.out_width, d.hidden
+    if tuple(dy.shape) != (*x.shape[:-1], O) or dy.dtype != x.dtype:
+        raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)}, expected {x.dtype} {(*x.shape[:-1], O)}")
+    _same_place(what, x, dy=dy, saved_gu=saved[0], saved_h=saved[1])
+    lib, hb = hip.load(), ctypes.c_int64()
+    gb = lib.cradle_gated_mlp_saved_bytes(M, F, d.dtype, ctypes.byref(hb))
+    if saved[0].numel() * 4 != gb or saved[1].numel() * 2 != hb.value:
+        raise hip.CradleHipError(f"{what}: the saved buffers do not belong to a block of these sizes")
+    make = torch.empty if M else torch.zeros
+    new = lambda *shape: make(shape, device=x.device, dtype=x.dtype)
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+    dw_in, dw_out = (new(2 * F, K) if need[1] else None), (new(O, F) if need[2] else None)
+    db_in, db_out = (new(2 * F), new(O)) if bias else (None, None)
+    if M:
+        dy2 = _rows_of(dy, what)
+        d.dy, d.ld_dy, d.saved_gu, d.saved_h = dy2.data_ptr(), _ld(dy2), saved[0].data_ptr(), saved[1].data_ptr()
+        d.dx, d.ld_dx, d.dw_in, d.dw_out, d.db_in, d.db_out = (_pointer(dx), K, _pointer(dw_in), _pointer(dw_out), _pointer(db_in),
+                                                               _pointer(db_out))
+        ws = _gated_workspace(d, 1, x.device)
+        with _on(x) as s:
+            hip.check(lib.cradle_gated_mlp_bwd(ctypes.byref(d), s), what)
+    return dx, dw_in, dw_out, db_in, db_out
+
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_bound(coeffs, steps: int) -> float:
+    """Largest magnitude that s and b s^2 + c s^4 take over the iteration s <- a s + b s^3 + c s^5 from any s in [0, 1]."""
+    a, b, c = (float(v) for v in coeffs)
+    s, most = torch.linspace(0, 1, 4097, dtype=torch.float64), 1.0
+    for _ in range(steps):
+        q = b * s * s + c * s ** 4
+        s = a * s + q * s
+        most = max(most, float(q.abs().max()), float(s.abs().max()))
+        if not most < 1e6:
+            return float("inf")
+        s = torch.linspace(0, float(s.abs().max()), 4097, dtype=torch.float64)  # (every value between: a superset)
+    return most
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of each matrix of ``g`` (..., m, n), fp32 / bf16 / fp16: X = G / (|G|_F + eps), then
+    ``steps`` times X <- a X + (b S + c S S) X with S = X X^T on the smaller side (``cradle_orthogonalize``); every singular value s
+    goes through a s + b s^3 + c s^5.  fp32 accuracy inside, one rounding to g's type.  ``out`` may be ``g``.  Coefficients
+    whose iteration leaves (-8, 8) from a start in [0, 1] are refused (the products hold X times 2^12 in fp16 planes)."""
+    what = "orthogonalize"
+    if not g.is_cuda or g.dtype not in FLOAT_TYPES or g.dim() < 2:
+        raise hip.CradleHipError(f"{what}: expected (..., m, n) fp32 / bf16 / fp16 on the GPU, got {g.dtype} {tuple(g.shape)} on {g.device}")
+    if not 1 <= int(steps) <= 64:
+        raise hip.CradleHipError(f"{what}: steps={steps} (1..64)")
+    coeffs = tuple(float(v) for v in coeffs)
+    if len(coeffs) != 3 or not _ns_bound(coeffs, int(steps)) < 8:
+        raise hip.CradleHipError(f"{what}: the iteration with coefficients {coeffs} does not stay within (-8, 8)")
+    m, n = g.shape[-2:]
+    if out is None:
+        out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    if out.shape != g.shape or out.dtype != g.dtype or out.device != g.device or not out.is_contiguous():
+        raise hip.CradleHipError(f"{what}: out must be contiguous and of g's shape, type and device")
+    if g.numel() == 0:
+        return out
+    g3 = g if g.dim() == 3 else g.unsqueeze(0) if g.dim() == 2 else g.reshape(-1, m, n)
+    if (n > 1 and g3.stride(2) != 1) or (m > 1 and g3.stride(1) < n) or g3.stride(0) < 0:
+        g3 = g3.contiguous()
+    B = g3.shape[0]
+    ld = g3.stride(1) if m > 1 else max(g3.stride(1), n)
+    lib = hip.load()
+    need = lib.cradle_orthogonalize_workspace_bytes(B, m, n)
+    if need < 0:
+        hip.check(1, "orthogonalize_workspace_bytes")
+    ws = torch.empty(need, device=g.device, dtype=torch.uint8)
+    with _on(g) as s:
+        hip.check(lib.cradle_orthogonalize(g3.data_ptr(), ld, g3.stride(0), out.data_ptr(), n, m * n, FLOAT_TYPES[g.dtype], B, m, n,
+                                           int(steps), *coeffs, float(eps), ws.data_ptr(), need, s), what)
     return out

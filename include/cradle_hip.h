@@ -418,6 +418,70 @@ int cradle_nb_sample_accumulate_ws(const float* logits, int64_t ld_logits, const
                                    int64_t workspace_floats, cradle_stream_t stream);
 int64_t cradle_nb_sample_workspace_floats(int P, int C, int G);
 
+/* ---- Normalised, gated hidden layers: no counterpart in the reference, whose layers are Linear + LeakyReLU + residual ------
+ * (cradle_vae/models/utils/mlp.py:83-119).  Tensors are fp32, bf16 or fp16 (CRADLE_F32 ...), rows contiguous with a leading
+ * dimension in elements; every sum, statistic and pre-activation is fp32 and a result is rounded once, to its tensor's type. */
+enum { CRADLE_F32 = 0, CRADLE_BF16 = 1, CRADLE_F16 = 2 };
+
+/* Layer norm over the last axis: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), var the mean squared
+ * deviation.  x (rows, width), y (rows, width); weight, bias (width) of type w_dtype (dtype or CRADLE_F32), NULL = 1 / 0;
+ * mean, rstd (rows) fp32, NULL = not kept.  1 <= width <= 32768. */
+int cradle_layer_norm_fwd(const void* x, int64_t ld_x, const void* weight, const void* bias, int dtype, int w_dtype, float eps,
+                          void* y, int64_t ld_y, float* mean, float* rstd, int64_t rows, int width, cradle_stream_t stream);
+/* Backward: dx (rows, width) or NULL; dweight, dbias (width, w_dtype) or NULL -- sums over the rows in a fixed order
+ * (deterministic), through `workspace`: cradle_layer_norm_workspace_floats(rows, width) floats, 16-byte aligned (may be NULL
+ * when neither is asked for). */
+int64_t cradle_layer_norm_workspace_floats(int64_t rows, int width);
+int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* weight, const float* mean,
+                          const float* rstd, int dtype, int w_dtype, void* dx, int64_t ld_dx, void* dweight, void* dbias,
+                          float* workspace, int64_t workspace_floats, int64_t rows, int width, cradle_stream_t stream);
+
+/* Gated feed-forward block: [g | u] = x W_in^T + b_in, h = act(g) * u, y = h W_out^T + b_out (+ residual).
+ * x (rows, width); w_in (2 hidden, width): the gate's rows, then the up projection's; w_out (out_width, hidden); b_in
+ * (2 hidden), b_out (out_width) or NULL; residual (rows, out_width) or NULL; y (rows, out_width).  act: 0 silu, 1 gelu (erf).
+ * Training: saved_gu and saved_h (cradle_gated_mlp_saved_bytes) receive what the backward pass reads; NULL for inference.
+ * cradle_gated_mlp_bwd: from dy (rows, out_width) and the saved buffers, dx (rows, width; NULL = not needed), dw_in, dw_out
+ * (contiguous, NULL = not needed), db_in, db_out (NULL = not needed).  The residual's gradient is dy.
+ * h and [dg | du] are rounded to the tensors' type where they enter a matrix product (fp32: to 24 bits).  fp32 inputs of
+ * magnitude above 3.39e38 count as infinite.  workspace: cradle_gated_mlp_workspace_bytes(desc, backward) bytes, 16-byte aligned;
+ * only the sizes, types, pointers' alignment and which pointers are NULL are read for it.
+ * hidden * ld_w_in < 2^30, widths <= 2^20, leading dimensions < 2^22. */
+typedef struct cradle_gated_mlp_desc {
+  int rows, width, hidden, out_width, dtype, act;
+  const void* x; int64_t ld_x;
+  const void* w_in; int64_t ld_w_in;
+  const void* w_out; int64_t ld_w_out;
+  const void* b_in;
+  const void* b_out;
+  const void* residual; int64_t ld_residual;
+  void* y; int64_t ld_y;
+  void* saved_gu;
+  void* saved_h;
+  const void* dy; int64_t ld_dy;
+  void* dx; int64_t ld_dx;
+  void* dw_in;
+  void* dw_out;
+  void* db_in;
+  void* db_out;
+  void* workspace; int64_t workspace_bytes;
+} cradle_gated_mlp_desc;
+/* bytes of saved_gu (returned) and of saved_h (*h_bytes) */
+int64_t cradle_gated_mlp_saved_bytes(int rows, int hidden, int dtype, int64_t* h_bytes);
+int64_t cradle_gated_mlp_workspace_bytes(const cradle_gated_mlp_desc* desc, int backward_pass);
+int cradle_gated_mlp_fwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stream);
+int cradle_gated_mlp_bwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stream);
+
+/* ---- Orthogonalised update of a weight matrix (an optimiser beside K10; no counterpart in the reference) -------------------
+ * For each of `batch` matrices G (m, n): X = G / (|G|_F + eps); `steps` times S = X X^T, X <- a X + (b S + c S S) X (on the
+ * smaller side); out = X.  g, out: CRADLE_F32 / BF16 / F16, rows contiguous, leading dimensions and batch strides in elements.
+ * fp32 accuracy throughout, one rounding to the output's type.  The polynomial s -> a s + b s^3 + c s^5, iterated from [0, 1],
+ * has to stay below 8 in magnitude together with b s^2 + c s^4 (the caller checks its coefficients; beyond 16 entries may
+ * overflow to infinity).  out may be g.  workspace: cradle_orthogonalize_workspace_bytes bytes, 16-byte aligned. */
+int64_t cradle_orthogonalize_workspace_bytes(int batch, int m, int n);
+int cradle_orthogonalize(const void* g, int64_t ld_g, int64_t batch_stride_g, void* out, int64_t ld_out, int64_t batch_stride_out,
+                         int dtype, int batch, int m, int n, int steps, float a, float b, float c, float eps, void* workspace,
+                         int64_t workspace_bytes, cradle_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
