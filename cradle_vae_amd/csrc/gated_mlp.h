@@ -44,32 +44,6 @@ __device__ __forceinline__ float act_only(int act, float g) {
   return cdf == 0.f ? 0.f : g * cdf;
 }
 
-__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
-  if (dtype == CRADLE_F32) return static_cast<const float*>(p)[i];
-  const u16 b = static_cast<const u16*>(p)[i];
-  return dtype == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
-}
-__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
-  if (dtype == CRADLE_F32) static_cast<float*>(p)[i] = v;
-  else static_cast<u16*>(p)[i] = dtype == CRADLE_BF16 ? bits_bf16(v) : bits_f16(v);
-}
-__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, f32x4 v, int n, bool vec) {
-  if (vec && n >= 4) {
-    if (dtype == CRADLE_F32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
-    } else {
-      u16 s[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = dtype == CRADLE_BF16 ? bits_bf16(v[e]) : bits_f16(v[e]);
-      *reinterpret_cast<u32x2*>(static_cast<u16*>(p) + i) = u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
-    }
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < n) store_as(p, i + e, dtype, v[e]);
-}
-
 // ---------------------------------------------------------------------------------------------------------------
 // packing: a tensor as operand planes with padded, zero-filled rows
 // ---------------------------------------------------------------------------------------------------------------
@@ -115,10 +89,13 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
 // ---------------------------------------------------------------------------------------------------------------
 // epilogues
 // ---------------------------------------------------------------------------------------------------------------
+struct NoState {};
+
 // h = act(g) u as operand planes (columns [hidden, ld) zero), g and u saved
 template <int ELEM, int NPH>
 struct GateEpi {
   static constexpr bool PAIR = true;
+  using State = NoState;
   int act, hidden, hidden_p;  // hidden_p: hidden rounded up to 8
   int dtype;
   const void* bias;  // (2 hidden) or NULL
@@ -126,11 +103,11 @@ struct GateEpi {
   int64_t h_plane;
   float* gu;  // (rows, 2 hidden_p) or NULL
   template <class T>
-  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
-                                        int) const {
-    each_piece<T, T::TN / 2>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
+    each_piece<T, T::WN / 2>(buf, lane, [&](int r, int c, const f32x4* p) {
+      const int m = m0 + r, n = n0 + c;
       if (m >= a.M || n >= hidden_p) return;
-      f32x4 g = quarter(acc[i][j], q), u = quarter(acc[i][j + T::TN / 2], q), h4;
+      f32x4 g = *p, u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + T::WN / 2), h4;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool in = n + e < hidden;
@@ -142,80 +119,72 @@ struct GateEpi {
       }
       store_planes<ELEM, NPH>(h + (int64_t)m * hidden_p + n, h_plane, h4);
       if (gu) {
-        float* r = gu + (int64_t)m * 2 * hidden_p + n;
-        *reinterpret_cast<f32x4*>(r) = g;
-        *reinterpret_cast<f32x4*>(r + hidden_p) = u;
+        float* o = gu + (int64_t)m * 2 * hidden_p + n;
+        *reinterpret_cast<f32x4*>(o) = g;
+        *reinterpret_cast<f32x4*>(o + hidden_p) = u;
       }
     });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
-
-// sum over the 32 lanes of a half wave; lanes 31 and 63 have it
-__device__ __forceinline__ float half_wave_sum(float v) {
-  v += dpp_move<0xB1, 0xF>(0.f, v);
-  v += dpp_move<0x4E, 0xF>(0.f, v);
-  v += dpp_move<0x141, 0xF>(0.f, v);
-  v += dpp_move<0x140, 0xF>(0.f, v);
-  v += dpp_move<0x142, 0xA>(0.f, v);
-  return v;
-}
 
 // acc = dh: dg = dh u act'(g), du = dh act(g) as operand planes side by side (rows of 2 hidden_p, padding zero), and, for the
 // bias gradient, their fp32 column sums over this wave's rows
+struct ColumnSums {
+  f32x4 g, u;
+};
 template <int ELEM, int NPD>
 struct GateBwdEpi {
   static constexpr bool PAIR = false;
+  using State = ColumnSums;
   int act, hidden, hidden_p;
   const float* gu;
   u16* d;  // (rows, 2 hidden_p)
   int64_t d_plane;
   float* partial;  // (tiles_m * WAVES_M, 2 hidden_p) or NULL
   template <class T>
-  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int tm, int,
-                                        int wm) const {
-    const int li = lane & 31, lh = lane >> 5;
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, ColumnSums& s, int, int) const {
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
+      const int m = m0 + r, n = n0 + c;
+      if (m >= a.M || n >= hidden_p) return;
+      const float* o = gu + (int64_t)m * 2 * hidden_p + n;
+      const f32x4 g = *reinterpret_cast<const f32x4*>(o), u = *reinterpret_cast<const f32x4*>(o + hidden_p), dh = *p;
+      f32x4 dg, du;
 #pragma unroll
-    for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + j * 32 + q * 8 + lh * 4;
-        f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < T::TM; ++i) {
-          const int m = m0 + i * 32 + li;
-          if (m < a.M && n < hidden_p) {
-            const float* r = gu + (int64_t)m * 2 * hidden_p + n;
-            const f32x4 g = *reinterpret_cast<const f32x4*>(r), u = *reinterpret_cast<const f32x4*>(r + hidden_p);
-            const f32x4 dh = quarter(acc[i][j], q);
-            f32x4 dg, du;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float av, dav;
-              act_both(act, g[e], av, dav);
-              const bool in = n + e < hidden;
-              dg[e] = in ? dh[e] * u[e] * dav : 0.f;
-              du[e] = in ? dh[e] * av : 0.f;
-            }
-            u16* o = d + (int64_t)m * 2 * hidden_p + n;
-            store_planes<ELEM, NPD>(o, d_plane, dg);
-            store_planes<ELEM, NPD>(o + hidden_p, d_plane, du);
-            sg += dg;
-            su += du;
-          }
-        }
-        if (partial) {
-          float* p = partial + (int64_t)(tm * T::WAVES_M + wm) * 2 * hidden_p + n;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sg[e] = half_wave_sum(sg[e]);
-            su[e] = half_wave_sum(su[e]);
-          }
-          if (li == 31 && n < hidden_p) {
-            *reinterpret_cast<f32x4*>(p) = sg;
-            *reinterpret_cast<f32x4*>(p + hidden_p) = su;
-          }
-        }
+      for (int e = 0; e < 4; ++e) {
+        float av, dav;
+        act_both(act, g[e], av, dav);
+        const bool in = n + e < hidden;
+        dg[e] = in ? dh[e] * u[e] * dav : 0.f;
+        du[e] = in ? dh[e] * av : 0.f;
       }
+      u16* q = d + (int64_t)m * 2 * hidden_p + n;
+      store_planes<ELEM, NPD>(q, d_plane, dg);
+      store_planes<ELEM, NPD>(q + hidden_p, d_plane, du);
+      s.g += dg;
+      s.u += du;
+    });
+  }
+  // a lane has seen the same four columns in every row it took: lanes a row's length apart hold the other rows
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int n0, int lane, ColumnSums& s, int tm, int wm) const {
+    if (!partial) return;
+    constexpr int P = T::WN / 4;
+    static_assert(P < 64 && 64 % P == 0, "columns of a wave");
+#pragma unroll
+    for (int k = P; k < 64; k *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s.g[e] += __shfl_xor(s.g[e], k);
+        s.u[e] += __shfl_xor(s.u[e], k);
+      }
+    const int n = n0 + lane * 4;
+    if (lane < P && n < hidden_p) {
+      float* o = partial + (int64_t)(tm * T::WAVES_M + wm) * 2 * hidden_p + n;
+      *reinterpret_cast<f32x4*>(o) = s.g;
+      *reinterpret_cast<f32x4*>(o + hidden_p) = s.u;
+    }
   }
 };
 
@@ -223,6 +192,7 @@ struct GateBwdEpi {
 // [dg | du]^T x); the padding rows are not stored.
 struct OutEpi {
   static constexpr bool PAIR = false;
+  using State = NoState;
   void* out;
   int64_t ld;
   int dtype;
@@ -247,27 +217,31 @@ struct OutEpi {
     store4(out, (int64_t)m * ld + n, dtype, v, left, vec);
   }
   template <class T>
-  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
-                                        int) const {
-    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
-      if (m < a.M && n < a.N) put(m, n, a.N, quarter(acc[i][j], q));
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
+      if (m0 + r < a.M && n0 + c < a.N) put(m0 + r, n0 + c, a.N, *p);
     });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
 // fp32 partial sums of a product split along K: (splits, M, Np), Np = N rounded up to 4
 struct PartialEpi {
   static constexpr bool PAIR = false;
+  using State = NoState;
   float* partial;
   int Np;
   template <class T>
-  __device__ __forceinline__ void store(const Args& a, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
-                                        int) const {
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
     float* base = partial + (int64_t)blockIdx.z * a.M * Np;
-    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
-      if (m < a.M && n < a.N) *reinterpret_cast<f32x4*>(base + (int64_t)m * Np + n) = quarter(acc[i][j], q);
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
+      const int m = m0 + r, n = n0 + c;
+      if (m < a.M && n < a.N) *reinterpret_cast<f32x4*>(base + (int64_t)m * Np + n) = *p;
     });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
 // joins the splits in order and finishes the output
@@ -281,32 +255,45 @@ static __global__ __launch_bounds__(256) void join_kernel(const float* __restric
   }
 }
 
-// column sums in two passes with a fixed order.  First: blockIdx.y-th share of the rows of a (rows, cols) tensor.
-static __global__ __launch_bounds__(256) void colsum_kernel(const void* __restrict__ src, int64_t ld, int dtype, int rows, int cols,
-                                                     int rows_per, float* __restrict__ partial) {
+// column sums in two passes with a fixed order.  First: blockIdx.y-th share of the rows of a (rows, cols) tensor, eight rows'
+// loads in flight per thread.
+template <int DT>
+static __global__ __launch_bounds__(256) void colsum_kernel(const void* __restrict__ src, int64_t ld, int rows, int cols, int rows_per,
+                                                            float* __restrict__ partial) {
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
   const int r1 = min(rows, (int)(blockIdx.y + 1) * rows_per);
   __shared__ float red[4][64];
   float s = 0.f;
   if (c < cols)
-    for (int r = blockIdx.y * rows_per + w; r < r1; r += 4) s += load_as(src, (int64_t)r * ld + c, dtype);
+    for (int r = blockIdx.y * rows_per + w; r < r1; r += 32) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = r + 4 * k < r1 ? load_as(src, (int64_t)(r + 4 * k) * ld + c, DT) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
   red[w][threadIdx.x & 63] = s;
   __syncthreads();
   if (w == 0 && c < cols)
     partial[(int64_t)blockIdx.y * cols + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 // Second: sums `n` partial rows of `ld` floats; columns [0, cols), of which those from gap_at on are read gap further right
-static __global__ __launch_bounds__(256) void colsum_join_kernel(const float* __restrict__ partial, int n, int ld, int cols, int gap_at,
-                                                          int gap, void* __restrict__ out, int dtype) {
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  __shared__ float red[4][64];
+static __global__ __launch_bounds__(1024) void colsum_join_kernel(const float* __restrict__ partial, int n, int ld, int cols,
+                                                                  int gap_at, int gap, void* __restrict__ out, int dtype) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  __shared__ float red[16][64];
   float s = 0.f;
-  if (c < cols)
-    for (int r = w; r < n; r += 4) s += partial[(int64_t)r * ld + c + (c >= gap_at ? gap : 0)];
-  red[w][threadIdx.x & 63] = s;
+  if (c < cols) {
+    const float* p = partial + c + (c >= gap_at ? gap : 0);
+#pragma unroll 4
+    for (int r = w; r < n; r += 16) s += p[(int64_t)r * ld];
+  }
+  red[w][lane] = s;
   __syncthreads();
-  if (w == 0 && c < cols)
-    store_as(out, c, dtype, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+  if (w != 0 || c >= cols) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) s += red[k][lane];
+  store_as(out, c, dtype, s);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -379,13 +366,13 @@ void run_pack(const Plan& p, PackJobs& js, int n_jobs, hipStream_t s) {
   hipLaunchKernelGGL((pack_kernel<ELEM, NPL>), grid, dim3(256), 0, s, js);
 }
 
-// Tiles: 256 x 256 (eight waves) when the product fills the chip with them, else 128 x 128 (four waves); three planes need
-// half the K step and, at the large size, half the columns to fit the LDS.
+// Two tiles per operand format.  Large: 256 x 256 (three planes: 256 x 128, to fit the LDS), eight waves, one workgroup per CU.
+// Small: 128 x 128 (three planes: 128 x 64), four waves, two workgroups per CU.
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
 struct Tiles {
   static constexpr bool ONE = NPA == 1 && NPB == 1;
-  using Large = Tile<ELEM, NPA, NPB, 256, ONE ? 256 : 128, ONE ? 64 : 32, ONE ? 2 : 4, ONE ? 4 : 2, AK, BK>;
-  using Small = Tile<ELEM, NPA, NPB, 128, 128, ONE ? 64 : 32, 2, 2, AK, BK>;
+  using Large = Tile<ELEM, NPA, NPB, 256, ONE ? 256 : 128, ONE ? 64 : 32, 2, ONE ? 2 : 4, ONE ? 4 : 2, AK, BK>;
+  using Small = Tile<ELEM, NPA, NPB, 128, ONE ? 128 : 64, ONE ? 64 : 32, 2, ONE ? 2 : 4, ONE ? 2 : 1, AK, BK>;
 };
 
 template <class T, class Epi>
@@ -405,27 +392,31 @@ int64_t tiles(const Args& a, int cols, bool pair) {
   return (int64_t)((a.M + T::BM - 1) / T::BM) * ((cols + bn - 1) / bn);
 }
 
-// large tiles pay while they leave no CU idle for long: at least one full wave of workgroups, the last one well filled
-inline bool use_large(int64_t n) { return n >= kCUs && (n % kCUs == 0 || n % kCUs >= kCUs / 2 || n >= 4 * kCUs); }
+// Time of a product on tiles of one size: the CUs with the most tiles finish last, a large tile's rate is 1.2 times a small
+// one's (measured on 8192 x 10240 x 4096 in bf16: 1290 and 1090 TFLOP/s).
+template <class L, class S>
+bool use_large(const Args& a, int cols, bool pair) {
+  const int64_t l = (tiles<L>(a, cols, pair) + kCUs - 1) / kCUs * L::BM * L::BN, s = (tiles<S>(a, cols, pair) + kCUs - 1) / kCUs * S::BM * S::BN;
+  return l * 5 <= s * 6;
+}
 
 template <int ELEM, int NPA, int NPB, bool AK, bool BK, class Epi>
 void product(const Args& a, const Epi& epi, int cols, hipStream_t s) {
   using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
-  if (use_large(tiles<typename TT::Large>(a, cols, Epi::PAIR))) launch<typename TT::Large>(a, epi, cols, 1, s);
+  if (use_large<typename TT::Large, typename TT::Small>(a, cols, Epi::PAIR)) launch<typename TT::Large>(a, epi, cols, 1, s);
   else launch<typename TT::Small>(a, epi, cols, 1, s);
 }
 
-// A product whose output has too few tiles for the chip is split along K, into shares of at least eight K tiles.
+// A product whose output has too few small tiles for the chip (two per CU at a time) is split along K, into shares of at
+// least four K tiles; its partial sums cost a pass over them, so the large tiles are only left for a real gain.
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
 int splits_of(const Args& a) {
   using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
-  if (use_large(tiles<typename TT::Large>(a, a.N, false))) return 1;
   const int64_t t = tiles<typename TT::Small>(a, a.N, false);
   const int k_tiles = (a.K + TT::Small::BK - 1) / TT::Small::BK;
-  int64_t want = (2 * kCUs + t - 1) / t;
-  const int most = k_tiles / 8;
-  if (t >= kCUs) want = 1;
-  return (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+  const int64_t want = 2 * kCUs / t, most = k_tiles / 4;
+  if (t >= kCUs || want < 2 || most < 2) return 1;
+  return (int)(want < most ? want : most);
 }
 
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
@@ -484,7 +475,7 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   return ws.off;
 }
 
-constexpr int kColsumRows = 256;  // rows per first-pass share of a column sum, more when there are more than 512 shares
+constexpr int kColsumRows = 64;  // rows per first-pass share of a column sum, more when there are more than 512 shares
 inline int colsum_rows(int rows) {
   const int most = (rows + 511) / 512;
   return most > kColsumRows ? most : kColsumRows;
@@ -509,7 +500,7 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   pf = pf > pf1 ? pf : pf1;
   pf = pf > pf2 ? pf : pf2;
   float* partial = static_cast<float*>(ws.take(pf * 4));
-  const int sum_rows = (p.M + 255) / 256 * 4;  // of either tile size: 256 rows are at most four wave rows
+  const int sum_rows = (p.M + 127) / 128 * 4;  // of either tile size: 128 rows are at most four wave rows
   float* sums = static_cast<float*>(ws.take(d->db_in ? (int64_t)sum_rows * 2 * p.Fp * 4 : 0));
   const int per = colsum_rows(p.M), shares = (p.M + per - 1) / per;
   float* sums_out = static_cast<float*>(ws.take(d->db_out ? (int64_t)shares * p.O * 4 : 0));
@@ -518,16 +509,17 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
 
   Args a = args_of(dy, w_out, p.M, p.F, p.O);
   using TT = Tiles<ELEM, NPL, NPL, true, false>;
-  const bool large = use_large(tiles<typename TT::Large>(a, p.F, false));
+  const bool large = use_large<typename TT::Large, typename TT::Small>(a, p.F, false);
   product<ELEM, NPL, NPL, true, false>(
       a, GateBwdEpi<ELEM, NPL>{d->act, p.F, p.Fp, static_cast<const float*>(d->saved_gu), dgu, d_plane, d->db_in ? sums : nullptr}, p.F, s);
   if (d->db_in) {
     const int used = large ? (p.M + 255) / 256 * TT::Large::WAVES_M : (p.M + 127) / 128 * TT::Small::WAVES_M;
-    hipLaunchKernelGGL(colsum_join_kernel, dim3((2 * p.F + 63) / 64), dim3(256), 0, s, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
+    hipLaunchKernelGGL(colsum_join_kernel, dim3((2 * p.F + 63) / 64), dim3(1024), 0, s, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
   }
   if (d->db_out) {
-    hipLaunchKernelGGL(colsum_kernel, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.dtype, p.M, p.O, per, sums_out);
-    hipLaunchKernelGGL(colsum_join_kernel, dim3((p.O + 63) / 64), dim3(256), 0, s, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
+    constexpr int DT = NPL == 3 ? CRADLE_F32 : ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
+    hipLaunchKernelGGL(colsum_kernel<DT>, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.M, p.O, per, sums_out);
+    hipLaunchKernelGGL(colsum_join_kernel, dim3((p.O + 63) / 64), dim3(1024), 0, s, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
   }
   const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
   const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};

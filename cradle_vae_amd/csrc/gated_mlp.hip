@@ -10,67 +10,69 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------
 // a few rows: dot products along the weights' rows, fp32 arithmetic
 // ---------------------------------------------------------------------------------------------------------------
-// One wave per weight row (a pair of rows, gate and up, for GATE), R rows of x at once; VEC elements per lane and load.
-template <int R, bool GATE>
-__global__ __launch_bounds__(256) void few_rows_kernel(const void* __restrict__ x, int64_t ldx, int x_dtype,
-                                                       const void* __restrict__ W, int64_t ldw, int dtype, int rows, int K, int N,
-                                                       const void* __restrict__ bias, int act, float* __restrict__ h,
-                                                       const void* __restrict__ res, int64_t ld_res, void* __restrict__ y,
-                                                       int64_t ldy, int vec) {
+// V consecutive numbers (16 bytes of a 16-bit or fp32 tensor)
+template <int DT>
+struct Piece {
+  static constexpr int V = DT == CRADLE_F32 ? 4 : 8;
+  u32x4 raw;
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (DT == CRADLE_F32) {
+      const uint32_t w = raw[e];  // (a copy: bit_cast of a vector's element takes the first one)
+      return __builtin_bit_cast(float, w);
+    }
+    const u16 b = (u16)(raw[e / 2] >> (e % 2 * 16));
+    return DT == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
+  }
+};
+
+// One wave per weight row (GATE: per pair of rows, gate and up), R rows of x (type XT) at once.  VEC: the weight is read in 16-byte
+// pieces, four in flight per lane and row; x comes from the caches, every wave reads all of it.
+template <int DT, int XT, int R, bool GATE, bool VEC>
+__global__ __launch_bounds__(256) void few_rows_kernel(const void* __restrict__ x, int64_t ldx, const void* __restrict__ W, int64_t ldw,
+                                                       int rows, int K, int N, const void* __restrict__ bias, int act,
+                                                       float* __restrict__ h, const void* __restrict__ res, int64_t ld_res,
+                                                       void* __restrict__ y, int64_t ldy) {
   const int lane = threadIdx.x & 63;
   const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
-  constexpr int NW = GATE ? 2 : 1;
+  constexpr int NW = GATE ? 2 : 1, V = VEC ? Piece<DT>::V : 1, U = 4;
+  constexpr int ES = DT == CRADLE_F32 ? 4 : 2;
+  const char* w0 = static_cast<const char*>(W) + (int64_t)n * ldw * ES;
+  const char* w1 = static_cast<const char*>(W) + (int64_t)(N + n) * ldw * ES;
   float acc[NW][R];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[w][r] = 0.f;
-  if (vec) {  // 16-byte pieces of W: 8 16-bit or 4 fp32 numbers
-    const int V = dtype == CRADLE_F32 ? 4 : 8;
-#pragma unroll 2
-    for (int k = lane * V; k < K; k += 64 * V) {
-      float wv[NW][8];
+  for (int k0 = lane * V; k0 < K; k0 += 64 * V * U) {
+    Piece<DT> p[U][NW];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 64 * V;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const int64_t row = (int64_t)(w ? N + n : n) * ldw;
-        if (dtype == CRADLE_F32) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(static_cast<const float*>(W) + row + k);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) wv[w][e] = t[e];
-        } else {
-          const u32x4 t = *reinterpret_cast<const u32x4*>(static_cast<const u16*>(W) + row + k);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u16 a = (u16)t[e], b = (u16)(t[e] >> 16);
-            wv[w][2 * e] = dtype == CRADLE_BF16 ? from_bf16(a) : from_f16(a);
-            wv[w][2 * e + 1] = dtype == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
-          }
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r >= rows) break;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e >= V) break;
-          const float xv = load_as(x, (int64_t)r * ldx + k + e, x_dtype);
-#pragma unroll
-          for (int w = 0; w < NW; ++w) acc[w][r] = fmaf(wv[w][e], xv, acc[w][r]);
+        p[u][w].raw = u32x4{0, 0, 0, 0};
+        if constexpr (VEC) {
+          if (k < K) p[u][w].raw = *reinterpret_cast<const u32x4*>((w ? w1 : w0) + (int64_t)k * ES);
+        } else if (k < K) {
+          if constexpr (DT == CRADLE_F32) p[u][w].raw[0] = *reinterpret_cast<const uint32_t*>((w ? w1 : w0) + (int64_t)k * ES);
+          else p[u][w].raw[0] = *reinterpret_cast<const u16*>((w ? w1 : w0) + (int64_t)k * ES);
         }
       }
     }
-  } else {
-    for (int k = lane; k < K; k += 64) {
-      float wv[NW];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) wv[w] = load_as(W, (int64_t)(w ? N + n : n) * ldw + k, dtype);
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 64 * V;
+      if (k >= K) break;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r >= rows) break;
-        const float xv = load_as(x, (int64_t)r * ldx + k, x_dtype);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) acc[w][r] = fmaf(wv[w], xv, acc[w][r]);
+        for (int e = 0; e < V; ++e) {
+          const float xv = load_as(x, (int64_t)r * ldx + k + e, XT);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) acc[w][r] = fmaf(p[u][w][e], xv, acc[w][r]);
+        }
       }
     }
   }
@@ -81,16 +83,36 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const void* __restrict__ 
     if constexpr (GATE) {
       float s1 = wave_sum(acc[1][r]);
       if (bias) {
-        s0 += load_as(bias, n, dtype);
-        s1 += load_as(bias, (int64_t)N + n, dtype);
+        s0 += load_as(bias, n, DT);
+        s1 += load_as(bias, (int64_t)N + n, DT);
       }
       if (lane == 0) h[(int64_t)r * N + n] = act_only(act, s0) * s1;
     } else if (lane == 0) {
-      if (bias) s0 += load_as(bias, n, dtype);
-      if (res) s0 += load_as(res, (int64_t)r * ld_res + n, dtype);
-      store_as(y, (int64_t)r * ldy + n, dtype, s0);
+      if (bias) s0 += load_as(bias, n, DT);
+      if (res) s0 += load_as(res, (int64_t)r * ld_res + n, DT);
+      store_as(y, (int64_t)r * ldy + n, DT, s0);
     }
   }
+}
+
+template <int DT, int R>
+void few_rows_run(const cradle_gated_mlp_desc* d, const Plan& p, hipStream_t s) {
+  float* h = static_cast<float*>(d->workspace);
+  constexpr int V = Piece<DT>::V;
+  const bool v1 = p.K % V == 0 && d->ld_w_in % V == 0 && ((uintptr_t)d->w_in & 15) == 0;
+  const bool v2 = p.F % V == 0 && d->ld_w_out % V == 0 && ((uintptr_t)d->w_out & 15) == 0;
+  auto up = v1 ? few_rows_kernel<DT, DT, R, true, true> : few_rows_kernel<DT, DT, R, true, false>;
+  auto down = v2 ? few_rows_kernel<DT, CRADLE_F32, R, false, true> : few_rows_kernel<DT, CRADLE_F32, R, false, false>;
+  hipLaunchKernelGGL(up, dim3((p.F + 3) / 4), dim3(256), 0, s, d->x, d->ld_x, d->w_in, d->ld_w_in, p.M, p.K, p.F, d->b_in, d->act, h,
+                     nullptr, (int64_t)0, nullptr, (int64_t)0);
+  hipLaunchKernelGGL(down, dim3((p.O + 3) / 4), dim3(256), 0, s, h, (int64_t)p.F, d->w_out, d->ld_w_out, p.M, p.F, p.O, d->b_out, 0,
+                     nullptr, d->residual, d->ld_residual, d->y, d->ld_y);
+}
+template <int R>
+void few_rows_by_type(const cradle_gated_mlp_desc* d, const Plan& p, hipStream_t s) {
+  if (p.dtype == CRADLE_F32) few_rows_run<CRADLE_F32, R>(d, p, s);
+  else if (p.dtype == CRADLE_BF16) few_rows_run<CRADLE_BF16, R>(d, p, s);
+  else few_rows_run<CRADLE_F16, R>(d, p, s);
 }
 
 int64_t forward_of(const cradle_gated_mlp_desc* d, const Plan& p, hipStream_t s, bool run) {
@@ -153,20 +175,8 @@ int cradle_gated_mlp_fwd(const cradle_gated_mlp_desc* d, cradle_stream_t s) {
                    "gated_mlp_fwd: workspace of %lld bytes (16-byte aligned) needed", (long long)need);
   const Plan p = plan_of(d);
   if (few_rows(d)) {
-    float* h = static_cast<float*>(d->workspace);
-    const int V = p.dtype == CRADLE_F32 ? 4 : 8;
-    const int v1 = p.K % V == 0 && d->ld_w_in % V == 0 && ((uintptr_t)d->w_in & 15) == 0;
-    const int v2 = p.F % V == 0 && d->ld_w_out % V == 0 && ((uintptr_t)d->w_out & 15) == 0;
-    const dim3 g1((p.F + 3) / 4), g2((p.O + 3) / 4);
-#define CRADLE_FEW(R)                                                                                                             \
-  {                                                                                                                               \
-    hipLaunchKernelGGL((few_rows_kernel<R, true>), g1, dim3(256), 0, s, d->x, d->ld_x, p.dtype, d->w_in, d->ld_w_in, p.dtype, p.M, \
-                       p.K, p.F, d->b_in, d->act, h, nullptr, 0, nullptr, 0, v1);                                                 \
-    hipLaunchKernelGGL((few_rows_kernel<R, false>), g2, dim3(256), 0, s, h, (int64_t)p.F, CRADLE_F32, d->w_out, d->ld_w_out,       \
-                       p.dtype, p.M, p.F, p.O, d->b_out, 0, nullptr, d->residual, d->ld_residual, d->y, d->ld_y, v2);              \
-  }
-    if (p.M == 1) CRADLE_FEW(1) else CRADLE_FEW(kFewRows)
-#undef CRADLE_FEW
+    if (p.M == 1) few_rows_by_type<1>(d, p, s);
+    else few_rows_by_type<kFewRows>(d, p, s);
   } else {
     forward_of(d, p, s, true);
   }

@@ -12,10 +12,11 @@
 // Orientation per operand: K-major ([row][k], k contiguous) or MN-major ([k][row], rows contiguous); the second is
 // transposed on its way from LDS to registers by ds_read_tr16_b64, so no transposed copy is ever made in memory.
 //
-// Staging: buffer loads straight into LDS, 16 bytes per lane, double-buffered; an element outside the operand is zero (its
+// Staging: buffer loads straight into LDS, 16 bytes per lane, two to four stages; an element outside the operand is zero (its
 // offset lies outside the buffer descriptor).  The LDS side of such a load is linear in the lane, so the layout that keeps
 // the fragment reads free of bank conflicts is made by permuting which 16-byte piece of a row a lane fetches:
-//   K-major : piece c of row r lies at c ^ swz(r), so that 8 (and 16) consecutive rows' pieces c fall into distinct banks;
+//   K-major : piece c of row r lies at c ^ swz(r), so that the rows a 16-byte read serves at once -- 16 consecutive ones, or four
+//             groups of four at 0, 12, 20, 24 (measured: the counter of bank conflicts) -- fall into distinct banks;
 //   MN-major: piece c of k-row k at c ^ 2 f(k & 3), f = {0,2,5,7} ({0,1,2,3} for 64 rows), so that the 4 x 32 bytes a 16-lane group transposes (and
 //             the two groups of a half wave) fall into distinct banks.
 //
@@ -42,6 +43,33 @@ __device__ __forceinline__ u16 bits_bf16(float v) { return __builtin_bit_cast(u1
 __device__ __forceinline__ u16 bits_f16(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
 __device__ __forceinline__ float from_bf16(u16 b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
 __device__ __forceinline__ float from_f16(u16 b) { return (float)__builtin_bit_cast(_Float16, b); }
+
+// one number of a tensor of type CRADLE_F32 / BF16 / F16
+__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
+  if (dtype == CRADLE_F32) return static_cast<const float*>(p)[i];
+  const u16 b = static_cast<const u16*>(p)[i];
+  return dtype == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+  if (dtype == CRADLE_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<u16*>(p)[i] = dtype == CRADLE_BF16 ? bits_bf16(v) : bits_f16(v);
+}
+__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, f32x4 v, int n, bool vec) {
+  if (vec && n >= 4) {
+    if (dtype == CRADLE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    } else {
+      u16 s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = dtype == CRADLE_BF16 ? bits_bf16(v[e]) : bits_f16(v[e]);
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p) + i) = u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) store_as(p, i + e, dtype, v[e]);
+}
 
 // v as NPL planes of ELEM numbers (round to nearest each).  A value that is not finite, or rounds to an infinity in the first
 // plane, keeps zeros in the others: the product is then an infinity or NaN in the rows and columns it belongs to.
@@ -71,23 +99,30 @@ struct Args {
   int symmetric;         // 1: only the tiles on and below the diagonal are computed (square tiles, tiles_m == tiles_n)
 };
 
-// Tile (BM x BN) of WAVES_M x WAVES_N waves, K step BK; operands of NPA and NPB planes of ELEM numbers.
-template <int ELEM_, int NPA_, int NPB_, int BM_, int BN_, int BK_, int WAVES_M_, int WAVES_N_, bool AK_, bool BKM_>
+// Tile (BM x BN) of WAVES_M x WAVES_N waves, K step BK, STAGES buffers in LDS; operands of NPA and NPB planes of ELEM numbers.
+template <int ELEM_, int NPA_, int NPB_, int BM_, int BN_, int BK_, int STAGES_, int WAVES_M_, int WAVES_N_, bool AK_, bool BKM_>
 struct Tile {
+  static constexpr int STAGES = STAGES_;
   static constexpr int ELEM = ELEM_, NPA = NPA_, NPB = NPB_, BM = BM_, BN = BN_, BK = BK_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_;
   static constexpr bool A_KMAJOR = AK_, B_KMAJOR = BKM_;
   static constexpr int NW = WAVES_M * WAVES_N, NT = 64 * NW;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
   static constexpr int CA = BM * BK / 8, CB = BN * BK / 8;  // 16-byte pieces per plane
   static constexpr int STAGE = NPA * CA + NPB * CB;
-  static constexpr int LDS_BYTES = 2 * STAGE * 16;
+  static constexpr int LDS_BYTES = STAGES * STAGE * 16;
+  static constexpr int LOADS = (NPA * CA + NPB * CB) / NT;    // per thread and stage
+  static constexpr int ROW = WN + 4;                          // floats of an epilogue row in LDS (the padding spreads the banks)
+  static constexpr int ROWS_BYTES = 32 * ROW * 4, ROWS_PER_STAGE = STAGE * 16 / ROWS_BYTES;
   static_assert(BK == 32 || BK == 64, "K step");
+  static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * LOADS < 64, "loads in flight");
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+  static_assert(ROWS_PER_STAGE * STAGES >= NW, "the waves' epilogue rows fit into the stages");
   static_assert(CA % NT == 0 && CB % NT == 0, "tile too small for the workgroup");
 };
 
 template <int BK>
 __device__ __forceinline__ int swz(int row) {
-  return BK == 64 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
+  return BK == 64 ? (row ^ (row >> 3)) & 7 : ((row >> 2) ^ (row & 16 ? 3 : 0)) & 3;
 }
 template <int ROWS>
 __device__ __forceinline__ int swz_k(int k) {
@@ -222,17 +257,54 @@ __device__ __forceinline__ void tile_of(const Args& a, int& tm, int& tn) {
   tn = in / rows;
 }
 
-// C tile = A B^T over this workgroup's K share, handed to the epilogue in registers: the second operand's rows are the MFMA's
-// first operand, so that four accumulator elements of a lane are four consecutive columns of one row (each_piece).
-// Epi::PAIR: a column's two halves are accumulators j and j + TN / 2 of the same lane.
+// orders the LDS accesses of one wave's lanes (they execute in order; the compiler must keep them so)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The W columns from c0 on of 32 epilogue rows in pieces of four, consecutive lanes consecutive pieces: fn(row, column, piece)
+template <class T, int W, class Fn>
+__device__ __forceinline__ void each_piece(float* buf, int lane, const Fn& fn) {
+  constexpr int P = W / 4;
+#pragma unroll
+  for (int it = 0; it < 32 * P / 64; ++it) {
+    const int idx = it * 64 + lane, r = idx / P, c = idx % P * 4;
+    fn(r, c, reinterpret_cast<f32x4*>(buf + r * T::ROW + c));
+  }
+}
+
+// The same, turned: four rows of one column, consecutive lanes consecutive rows: fn(first row, column, numbers)
+template <class T, int W, class Fn>
+__device__ __forceinline__ void each_turned_piece(const float* buf, int lane, const Fn& fn) {
+#pragma unroll
+  for (int it = 0; it < W / 8; ++it) {
+    const int r = lane % 8 * 4, c = it * 8 + lane / 8;
+    fn(r, c, f32x4{buf[r * T::ROW + c], buf[(r + 1) * T::ROW + c], buf[(r + 2) * T::ROW + c], buf[(r + 3) * T::ROW + c]});
+  }
+}
+
+// C tile = A B^T over this workgroup's K share.  Loads run STAGES K tiles ahead of the products and fragments one MFMA step (16
+// of K) ahead: before its last MFMA step a K tile waits for the next stage's loads (s_waitcnt vmcnt of the later stages' count), then
+// for the other waves -- whose fragments of this stage are in registers by then --, refills this stage and fetches the next
+// one's first fragments, all of it under the products still to come.  The stages are separate arrays and the loop is unrolled
+// over them, so that the compiler can tell the buffer being filled from the one being read and adds no wait of its own.
+// The second operand's rows are the MFMA's first operand: four accumulator elements of a lane are four consecutive columns of
+// one row.  The epilogue gets the tile 32 rows of a wave at a time, turned through LDS so that consecutive lanes hold
+// consecutive pieces of a row: its loads and stores then cover whole cache lines.
+// Epi: emit(a, buf, m0, n0, lane, state, tm, tn) for every 32 rows, finish(...) once; Epi::PAIR: columns [0, WN / 2) of buf are the
+// first half's, [WN / 2, WN) the second's.
 template <class T, class Epi>
 __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const Epi epi) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass only needs the launch stub; with the body it leaves some of them out)
   static_assert(!Epi::PAIR || T::TN % 2 == 0, "a wave holds both halves of a column");
   using SA = Stager<T, T::A_KMAJOR, T::BM, T::NPA>;
   using SB = Stager<T, T::B_KMAJOR, T::BN, T::NPB>;
+  constexpr int S = T::STAGES;
   __shared__ u32x4 st0[T::STAGE];
   __shared__ u32x4 st1[T::STAGE];
+  __shared__ u32x4 st2[S > 2 ? T::STAGE : 1];
+  __shared__ u32x4 st3[S > 3 ? T::STAGE : 1];
   int tm, tn;
   tile_of(a, tm, tn);
   const int row0 = tm * T::BM, col0 = tn * (Epi::PAIR ? T::BN / 2 : T::BN);
@@ -247,84 +319,127 @@ __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const E
   const int k_tiles = (a.K + T::BK - 1) / T::BK;
   const int kt0 = blockIdx.z * a.k_tiles_per_split, kt1 = min(k_tiles, kt0 + a.k_tiles_per_split);
 
-  f32x16 acc[T::TM][T::TN];
+  // Where the registers allow, the products of lower planes are summed apart: in one accumulator each of them would be rounded
+  // at the size of the whole sum (six roundings per 16 of K instead of one).
+  constexpr bool APART = (T::NPA > 1 || T::NPB > 1) && T::TM * T::TN <= 4;
+  f32x16 acc[T::TM][T::TN], low[APART ? T::TM : 1][APART ? T::TN : 1];
 #pragma unroll
   for (int i = 0; i < T::TM; ++i)
 #pragma unroll
     for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < 16; ++e) {
+        acc[i][j][e] = 0.f;
+        if constexpr (APART) low[i][j][e] = 0.f;
+      }
 
+  // (beyond the share's last tile every piece lies outside: the count of loads in flight stays the same)
   auto issue = [&](u32x4* st, int kt) {
-    sa.issue(a.A, st, kt * T::BK);
-    sb.issue(a.B, st + T::NPA * T::CA, kt * T::BK);
+    const int k0 = kt < kt1 ? kt * T::BK : 0x40000000;
+    sa.issue(a.A, st, k0);
+    sb.issue(a.B, st + T::NPA * T::CA, k0);
   };
-  auto wait_all = [&]() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+  auto barrier = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
-  // products of one stage; the next stage's loads are issued once this stage's first fragments are on their way
-  auto step = [&](const u32x4* cur, u32x4* nxt, int kt_next) {
-    const u32x4* ca = cur;
-    const u32x4* cb = cur + T::NPA * T::CA;
-    if (kt_next < kt1) issue(nxt, kt_next);
+  u32x4 fa[2][T::NPA][T::TM], fb[2][T::NPB][T::TN];
+  auto fetch = [&](const u32x4* st, int kk, int f) {
+    const u32x4* ca = st;
+    const u32x4* cb = st + T::NPA * T::CA;
+#pragma unroll
+    for (int p = 0; p < T::NPA; ++p)
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i) fa[f][p][i] = SA::frag(ca + p * T::CA, wm * T::WM + i * 32, kk, lane);
+#pragma unroll
+    for (int p = 0; p < T::NPB; ++p)
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j) fb[f][p][j] = SB::frag(cb + p * T::CB, wn * T::WN + j * 32, kk, lane);
+  };
+  // planes pa + pb < max(NPA, NPB), the smallest products first
+  auto multiply = [&](int f) {
+#pragma unroll
+    for (int s = (T::NPA > T::NPB ? T::NPA : T::NPB) - 1; s >= 0; --s)
+#pragma unroll
+      for (int pa = T::NPA - 1; pa >= 0; --pa) {
+        const int pb = s - pa;
+        if (pb < 0 || pb >= T::NPB) continue;
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < T::TN; ++j) {
+            f32x16& c = APART && s > 0 ? low[APART ? i : 0][APART ? j : 0] : acc[i][j];
+            c = mfma<T::ELEM>(fb[f][pb][j], fa[f][pa][i], c);
+          }
+      }
+  };
+  auto step = [&](u32x4* cur, const u32x4* nxt, int kt) {
 #pragma unroll
     for (int kk = 0; kk < T::BK / 16; ++kk) {
-      u32x4 fa[T::NPA][T::TM], fb[T::NPB][T::TN];
-#pragma unroll
-      for (int p = 0; p < T::NPA; ++p)
-#pragma unroll
-        for (int i = 0; i < T::TM; ++i) fa[p][i] = SA::frag(ca + p * T::CA, wm * T::WM + i * 32, kk, lane);
-#pragma unroll
-      for (int p = 0; p < T::NPB; ++p)
-#pragma unroll
-        for (int j = 0; j < T::TN; ++j) fb[p][j] = SB::frag(cb + p * T::CB, wn * T::WN + j * 32, kk, lane);
-      // planes pa + pb < max(NPA, NPB), the smallest products first
-#pragma unroll
-      for (int s = (T::NPA > T::NPB ? T::NPA : T::NPB) - 1; s >= 0; --s)
-#pragma unroll
-        for (int pa = T::NPA - 1; pa >= 0; --pa) {
-          const int pb = s - pa;
-          if (pb < 0 || pb >= T::NPB) continue;
-#pragma unroll
-          for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-            for (int j = 0; j < T::TN; ++j) acc[i][j] = mfma<T::ELEM>(fb[pb][j], fa[pa][i], acc[i][j]);
-        }
+      if (kk + 1 < T::BK / 16) {
+        fetch(cur, kk + 1, (kk + 1) & 1);
+      } else {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
+        barrier();
+        issue(cur, kt + S);
+        fetch(nxt, 0, 0);
+      }
+      multiply(kk & 1);
     }
-    wait_all();
   };
 
-  if (kt0 < kt1) {
-    issue(st0, kt0);
-    wait_all();
-    for (int kt = kt0; kt < kt1; kt += 2) {
-      step(st0, st1, kt + 1);
-      if (kt + 1 < kt1) step(st1, st0, kt + 2);
+  issue(st0, kt0);
+  issue(st1, kt0 + 1);
+  if constexpr (S > 2) issue(st2, kt0 + 2);
+  if constexpr (S > 3) issue(st3, kt0 + 3);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * T::LOADS) : "memory");
+  barrier();
+  fetch(st0, 0, 0);
+  for (int kt = kt0; kt < kt1; kt += S) {
+    step(st0, st1, kt);
+    if constexpr (S == 2) {
+      if (kt + 1 < kt1) step(st1, st0, kt + 1);
+    } else {
+      if (kt + 1 < kt1) step(st1, st2, kt + 1);
+      if constexpr (S == 3) {
+        if (kt + 2 < kt1) step(st2, st0, kt + 2);
+      } else {
+        if (kt + 2 < kt1) step(st2, st3, kt + 2);
+        if (kt + 3 < kt1) step(st3, st0, kt + 3);
+      }
     }
   }
+  if constexpr (APART) {
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j) acc[i][j] += low[i][j];
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  barrier();
 
-  epi.template store<T>(a, acc, row0 + wm * T::WM, col0 + wn * (Epi::PAIR ? T::WN / 2 : T::WN), lane, tm, tn, wm);
-#endif
-}
-
-// Walks a wave's accumulators in pieces of four consecutive columns: fn(i, m, j, q, n).  m, n: first row / column of the wave.
-template <class T, int TN, class Fn>
-__device__ __forceinline__ void each_piece(int m0, int n0, int lane, const Fn& fn) {
+  // this wave's 32 epilogue rows lie in one of the stages, which nobody reads any more
+  const int slot = wave / T::ROWS_PER_STAGE, in = wave % T::ROWS_PER_STAGE;
+  u32x4* st = slot == 0 ? st0 : slot == 1 ? st1 : slot == 2 ? st2 : st3;
+  float* buf = reinterpret_cast<float*>(st) + in * 32 * T::ROW;
   const int li = lane & 31, lh = lane >> 5;
+  const int m0 = row0 + wm * T::WM, n0 = col0 + wn * (Epi::PAIR ? T::WN / 2 : T::WN);
+  typename Epi::State state{};
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i)
+  for (int i = 0; i < T::TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) fn(i, m0 + i * 32 + li, j, q, n0 + j * 32 + q * 8 + lh * 4);
-}
-template <int Q>
-__device__ __forceinline__ f32x4 quarter(const f32x16& c) {
-  return f32x4{c[4 * Q], c[4 * Q + 1], c[4 * Q + 2], c[4 * Q + 3]};
-}
-__device__ __forceinline__ f32x4 quarter(const f32x16& c, int q) {
-  return q == 0 ? quarter<0>(c) : q == 1 ? quarter<1>(c) : q == 2 ? quarter<2>(c) : quarter<3>(c);
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(buf + li * T::ROW + j * 32 + q * 8 + lh * 4) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    wave_sync();
+    epi.template emit<T>(a, buf, m0 + i * 32, n0, lane, state, tm, tn);
+    wave_sync();
+  }
+  epi.template finish<T>(a, n0, lane, state, tm, wm);
+#endif
 }
 
 // four numbers as NPL planes at p (8-byte aligned; the planes lie `plane` elements apart)

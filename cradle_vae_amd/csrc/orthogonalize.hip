@@ -18,18 +18,7 @@ namespace {
 using namespace mm16;
 
 constexpr float kScale = 4096.f;  // X, S, B are held times this
-constexpr int kNormBlocks = 64;
 constexpr int kCUs = 256;
-
-__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
-  if (dtype == CRADLE_F32) return static_cast<const float*>(p)[i];
-  const u16 b = static_cast<const u16*>(p)[i];
-  return dtype == CRADLE_BF16 ? from_bf16(b) : from_f16(b);
-}
-__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
-  if (dtype == CRADLE_F32) static_cast<float*>(p)[i] = v;
-  else static_cast<u16*>(p)[i] = dtype == CRADLE_BF16 ? bits_bf16(v) : bits_f16(v);
-}
 
 struct Tensor {
   const void* p;
@@ -37,35 +26,57 @@ struct Tensor {
   int dtype, rows, cols;
 };
 
-// partial sums of squares, (batch, kNormBlocks) doubles
+// partial sums of squares, (batch, gridDim.x) doubles: a wave takes every 4 gridDim.x-th row, 16 bytes per lane where rows allow
+template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void sumsq_kernel(const Tensor g, double* __restrict__ part) {
   __shared__ double red[4];
-  const int64_t base = (int64_t)blockIdx.y * g.batch;
-  const int r0 = (int)((int64_t)g.rows * blockIdx.x / kNormBlocks), r1 = (int)((int64_t)g.rows * (blockIdx.x + 1) / kNormBlocks);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int V = !VEC ? 1 : DT == CRADLE_F32 ? 4 : 8, ES = DT == CRADLE_F32 ? 4 : 2;
+  // (a row in parts of 4096 elements, so that a few long rows are shared out too)
+  const int parts = (g.cols + 4095) / 4096;
+  const int64_t items = (int64_t)g.rows * parts;
   double s = 0;
-  const int64_t total = (int64_t)(r1 - r0) * g.cols;
-  int r = r0 + (int)(threadIdx.x / (unsigned)g.cols), c = (int)(threadIdx.x % (unsigned)g.cols);
-  const int dr = 256 / g.cols, dc = 256 % g.cols;
-  for (int64_t t = threadIdx.x; t < total; t += 256) {
-    const double v = load_as(g.p, base + (int64_t)r * g.ld + c, g.dtype);
-    s += v * v;
-    c += dc;
-    r += dr;
-    if (c >= g.cols) c -= g.cols, ++r;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < items; t += (int64_t)gridDim.x * 4) {
+    const int64_t row = (int64_t)blockIdx.y * g.batch + (t / parts) * g.ld;
+    const int c0 = (int)(t % parts) * 4096, c1 = min(g.cols, c0 + 4096);
+    float f = 0.f;
+    double d = 0;
+#pragma unroll 4
+    for (int c = c0 + lane * V; c < c1; c += 64 * V) {
+      if constexpr (VEC) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const char*>(g.p) + (row + c) * ES);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t bits = w[DT == CRADLE_F32 ? e : 0];  // (a copy: bit_cast of a vector's element takes the first one)
+          const float v = DT == CRADLE_F32 ? __builtin_bit_cast(float, bits)
+                          : DT == CRADLE_BF16 ? from_bf16((u16)(w[e / 2] >> (e % 2 * 16))) : from_f16((u16)(w[e / 2] >> (e % 2 * 16)));
+          if constexpr (DT == CRADLE_F16) f = fmaf(v, v, f);  // (64 squares below 2^32 each: no overflow)
+          else d += (double)v * v;
+        }
+      } else {
+        const float v = load_as(g.p, row + c, DT);
+        if constexpr (DT == CRADLE_F16) f = fmaf(v, v, f);
+        else d += (double)v * v;
+      }
+    }
+    s += d + f;
   }
   for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  if (lane == 0) red[wave] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * kNormBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // X (times kScale) as two planes of rows x ldx, rows <= columns: G or its transpose.  64 x 64 tiles through LDS.
-__global__ __launch_bounds__(256) void pack_kernel(const Tensor g, const double* __restrict__ part, float eps, int flip, u16* __restrict__ x,
-                                                   int64_t plane, int64_t batch, int m, int n, int ldx) {
+__global__ __launch_bounds__(256) void pack_kernel(const Tensor g, const double* __restrict__ part, int parts, float eps, int flip,
+                                                   u16* __restrict__ x, int64_t plane, int64_t batch, int m, int n, int ldx) {
   __shared__ float tile[64][65];
-  double s = 0;
-#pragma unroll 8
-  for (int k = 0; k < kNormBlocks; ++k) s += part[(int64_t)blockIdx.z * kNormBlocks + k];
+  __shared__ double red[4];
+  double s = (int)threadIdx.x < parts ? part[(int64_t)blockIdx.z * parts + threadIdx.x] : 0.0;  // (parts <= 256)
+  for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = (red[0] + red[1]) + (red[2] + red[3]);
   const float scale = kScale / ((float)sqrt(s) + eps);
   const int64_t base = (int64_t)blockIdx.z * g.batch;
   const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;  // of X
@@ -93,72 +104,84 @@ __device__ __forceinline__ f32x4 load_planes(const u16* p, int64_t plane) {
                from_f16((u16)h.y) + from_f16((u16)l.y), from_f16((u16)(h.y >> 16)) + from_f16((u16)(l.y >> 16))};
 }
 
-// out = alpha acc + beta add, a symmetric matrix of `size` rows, ld = size rounded up to 8 (padding columns zero)
+struct NoState {};
+
+// out = alpha acc + beta add, a symmetric matrix of `size` rows, ld = size rounded up to 8 (padding columns zero).  Tiles below the
+// diagonal are stored a second time, turned, above it.
 struct SymEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
+  using State = NoState;
   float alpha, beta;
   const u16* add;  // or NULL
   u16* out;
   int64_t plane, batch;
   int size, ld;
-  __device__ __forceinline__ void put(int m, int n, f32x4 v, bool mirror) const {
-    const int64_t b = (int64_t)blockIdx.y * batch;
+  __device__ __forceinline__ f32x4 value(int m, int n, f32x4 v) const {
     v *= alpha;
-    if (m < size) {
-      if (add) v += beta * load_planes(add + b + (int64_t)m * ld + n, plane);
-      store_planes<F16, 2>(out + b + (int64_t)m * ld + n, plane, v);
-    }
-    if (mirror && m < ld) {  // (rows beyond the matrix: the zero padding of the mirrored rows)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= size) break;
-        u16 s[2];
-        split<F16, 2>(v[e], s);
-        u16* o = out + b + (int64_t)(n + e) * ld + m;
-        o[0] = s[0];
-        o[plane] = s[1];
-      }
-    }
+    if (m < size && n < ld && add) v += beta * load_planes(add + (int64_t)blockIdx.y * batch + (int64_t)m * ld + n, plane);
+    return v;
+  }
+  __device__ __forceinline__ void put(int row, int col, f32x4 v) const {
+    if (row < size && col < ld) store_planes<F16, 2>(out + (int64_t)blockIdx.y * batch + (int64_t)row * ld + col, plane, v);
   }
   template <class T>
-  __device__ __forceinline__ void store(const Args&, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int tm, int tn,
-                                        int) const {
-    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
-      if (n < ld) put(m, n, quarter(acc[i][j], q), tm != tn);
+  __device__ __forceinline__ void emit(const Args&, float* buf, int m0, int n0, int lane, NoState&, int tm, int tn) const {
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4* p) {
+      const f32x4 v = value(m0 + r, n0 + c, *p);
+      put(m0 + r, n0 + c, v);
+      *p = v;
     });
+    if (tm == tn) return;
+    wave_sync();
+    each_turned_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4 v) { put(n0 + c, m0 + r, v); });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
 // fp32 partial sums of a symmetric product split along K: (split, batch, size, ld)
 struct SymPartialEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
+  using State = NoState;
   float* partial;
   int size, ld;
   template <class T>
-  __device__ __forceinline__ void store(const Args&, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int, int) const {
+  __device__ __forceinline__ void emit(const Args&, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
     float* base = partial + ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * size * ld;
-    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
-      if (m < size && n < ld) *reinterpret_cast<f32x4*>(base + (int64_t)m * ld + n) = quarter(acc[i][j], q);
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
+      const int m = m0 + r, n = n0 + c;
+      if (m < size && n < ld) *reinterpret_cast<f32x4*>(base + (int64_t)m * ld + n) = *p;
     });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 // joins the splits of the tiles on and below the diagonal, one workgroup per 32 x 32 block of the result
 __global__ __launch_bounds__(256) void sym_join_kernel(const float* __restrict__ partial, int splits, int tile, const SymEpi epi) {
+  __shared__ float turned[32][33];
   const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
-  const int m = blockIdx.z * 32 + r, n = blockIdx.x * 32 + c;
-  if (n / tile > m / tile || n >= epi.ld) return;
+  const int m0 = blockIdx.z * 32, n0 = blockIdx.x * 32, m = m0 + r, n = n0 + c;
+  if (n0 / tile > m0 / tile) return;  // (tiles are multiples of 32: the whole workgroup)
   const int64_t per = (int64_t)gridDim.y * epi.size * epi.ld;
   f32x4 v = {0, 0, 0, 0};
-  if (m < epi.size) {
+  if (m < epi.size && n < epi.ld) {
     const float* p = partial + ((int64_t)blockIdx.y * epi.size + m) * epi.ld + n;
+#pragma unroll 4
     for (int z = 0; z < splits; ++z) v += *reinterpret_cast<const f32x4*>(p + z * per);
   }
-  epi.put(m, n, v, n / tile != m / tile);
+  v = epi.value(m, n, v);
+  epi.put(m, n, v);
+  if (n0 / tile == m0 / tile) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) turned[c + e][r] = v[e];
+  __syncthreads();
+  epi.put(n0 + r, m0 + c, f32x4{turned[r][c], turned[r][c + 1], turned[r][c + 2], turned[r][c + 3]});
 }
 
-// X' = a X + B X as planes, or (last step) the result itself, transposed back where G was
+// X' = a X + B X as planes, or (last step) the result itself, turned back where G was
 struct StepEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
+  using State = NoState;
   float a, alpha;
   const u16* x;
   u16* out;
@@ -166,24 +189,26 @@ struct StepEpi {
   int ld;
   void* result;  // or NULL
   int64_t ld_result, batch_result;
-  int dtype, flip;
+  int dtype, flip, vec;
   template <class T>
-  __device__ __forceinline__ void store(const Args& ar, const f32x16 (&acc)[T::TM][T::TN], int m0, int n0, int lane, int, int,
-                                        int) const {
+  __device__ __forceinline__ void emit(const Args& ar, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
     const int64_t b = (int64_t)blockIdx.y * batch, br = (int64_t)blockIdx.y * batch_result;
-    each_piece<T, T::TN>(m0, n0, lane, [&](int i, int m, int j, int q, int n) {
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4* p) {
+      const int m = m0 + r, n = n0 + c;
       if (m >= ar.M || n >= ld) return;
-      const f32x4 v = alpha * quarter(acc[i][j], q) + a * load_planes(x + b + (int64_t)m * ld + n, plane);
-      if (!result) {
-        store_planes<F16, 2>(out + b + (int64_t)m * ld + n, plane, v);
-        return;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < ar.N)
-          store_as(result, br + (flip ? (int64_t)(n + e) * ld_result + m : (int64_t)m * ld_result + n + e), dtype, v[e] * (1.f / kScale));
+      const f32x4 v = alpha * *p + a * load_planes(x + b + (int64_t)m * ld + n, plane);
+      if (!result) store_planes<F16, 2>(out + b + (int64_t)m * ld + n, plane, v);
+      else if (flip) *p = v * (1.f / kScale);
+      else store4(result, br + (int64_t)m * ld_result + n, dtype, v * (1.f / kScale), ar.N - n, vec);
+    });
+    if (!result || !flip) return;
+    wave_sync();
+    each_turned_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4 v) {
+      if (n0 + c < ar.N && m0 + r < ar.M) store4(result, br + (int64_t)(n0 + c) * ld_result + m0 + r, dtype, v, ar.M - m0 - r, vec);
     });
   }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -194,9 +219,9 @@ inline int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 // three tile sizes: the largest whose tiles still occupy the chip
 template <bool BK>
 struct Tiles {
-  using Large = Tile<F16, 2, 2, 256, 256, 32, 2, 4, true, BK>;
-  using Medium = Tile<F16, 2, 2, 128, 128, 32, 2, 2, true, BK>;
-  using Small = Tile<F16, 2, 2, 64, 64, 64, 2, 2, true, BK>;
+  using Large = Tile<F16, 2, 2, 256, 256, 32, 2, 2, 4, true, BK>;
+  using Medium = Tile<F16, 2, 2, 128, 128, 32, 2, 2, 2, true, BK>;
+  using Small = Tile<F16, 2, 2, 64, 64, 64, 2, 2, 2, true, BK>;
 };
 
 inline int64_t tile_count(int64_t M, int64_t N, int t, bool sym) {
@@ -237,7 +262,7 @@ void product(const Args& a, const Epi& epi, int cols, int batch, int tile, int s
 struct Layout {
   int64_t x_plane, s_plane, x_batch, s_batch;  // elements
   int64_t norm, x0, x1, sm, bm, partial, total;  // byte offsets
-  int ldx, lds, tile_s, splits;
+  int ldx, lds, tile_s, splits, parts;
 };
 inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 Layout layout_of(int64_t batch, int64_t m, int64_t n) {  // m <= n
@@ -253,7 +278,9 @@ Layout layout_of(int64_t batch, int64_t m, int64_t n) {  // m <= n
     o += align256(bytes);
     return r;
   };
-  l.norm = take(batch * kNormBlocks * 8);
+  // workgroups of the norm: 16 K elements each, at most 256 per matrix
+  l.parts = (int)((m * n + 16383) / 16384 < 256 ? (m * n + 16383) / 16384 : 256);
+  l.norm = take(batch * l.parts * 8);
   l.x0 = take(batch * l.x_batch * 2);
   l.x1 = take(batch * l.x_batch * 2);
   l.sm = take(batch * l.s_batch * 2);
@@ -300,9 +327,15 @@ int cradle_orthogonalize(const void* g, int64_t ld_g, int64_t batch_stride_g, vo
   u16 *sm = reinterpret_cast<u16*>(w + l.sm), *bm = reinterpret_cast<u16*>(w + l.bm);
   float* partial = reinterpret_cast<float*>(w + l.partial);
   const Tensor gt{g, ld_g, batch_stride_g, dtype, m, n};
-  hipLaunchKernelGGL(sumsq_kernel, dim3(kNormBlocks, batch), dim3(256), 0, s, gt, norm);
-  hipLaunchKernelGGL(pack_kernel, dim3((N + 63) / 64, (M + 63) / 64, batch), dim3(256), 0, s, gt, norm, eps, (int)flip, x, l.x_plane,
+  const int V = dtype == CRADLE_F32 ? 4 : 8;
+  const bool vec = n % V == 0 && ld_g % V == 0 && batch_stride_g % V == 0 && ((uintptr_t)g & 15) == 0;
+  auto sumsq = dtype == CRADLE_F32    ? (vec ? sumsq_kernel<CRADLE_F32, true> : sumsq_kernel<CRADLE_F32, false>)
+               : dtype == CRADLE_BF16 ? (vec ? sumsq_kernel<CRADLE_BF16, true> : sumsq_kernel<CRADLE_BF16, false>)
+                                      : (vec ? sumsq_kernel<CRADLE_F16, true> : sumsq_kernel<CRADLE_F16, false>);
+  hipLaunchKernelGGL(sumsq, dim3(l.parts, batch), dim3(256), 0, s, gt, norm);
+  hipLaunchKernelGGL(pack_kernel, dim3((N + 63) / 64, (M + 63) / 64, batch), dim3(256), 0, s, gt, norm, l.parts, eps, (int)flip, x, l.x_plane,
                      l.x_batch, M, N, l.ldx);
+  const int vec_out = ld_out % 4 == 0 && batch_stride_out % 4 == 0 && ((uintptr_t)out & (dtype == CRADLE_F32 ? 15 : 7)) == 0;
   const int tile_x = pick_tile(M, N, batch, false);
   for (int k = 0; k < steps; ++k) {
     const Operand xo{x, l.ldx, l.x_plane, l.x_batch}, so{sm, l.lds, l.s_plane, l.s_batch}, bo{bm, l.lds, l.s_plane, l.s_batch};
@@ -321,7 +354,7 @@ int cradle_orthogonalize(const void* g, int64_t ld_g, int64_t batch_stride_g, vo
     ar.A = bo, ar.B = xo, ar.N = N;
     const bool last = k + 1 == steps;
     product<false>(ar, StepEpi{a, 1.f / kScale, x, x_next, l.x_plane, l.x_batch, l.ldx, last ? out : nullptr, ld_out, batch_stride_out, dtype,
-                               (int)flip},
+                               (int)flip, vec_out},
                    N, batch, tile_x, 1, false, s);
     u16* t = x;
     x = x_next;
