@@ -53,15 +53,17 @@ struct PackJob {
   int64_t ld_src, plane;
   int rows, cols, rows_dst, ld_dst;
   int gap_at, gap;  // destination rows [gap_at, gap_at + gap) are zero, and so are those behind the source's last
+  int vec;          // fp32 source with 16-byte aligned rows
 };
 struct PackJobs {
   PackJob job[4];
-  int dtype;
 };
 
-// one thread per 8 destination elements; ELEM planes
+// one thread per 8 destination elements; ELEM planes.  DT: the source's type; rows with a 16-byte aligned start are read in
+// 16-byte pieces.
 template <int ELEM, int NPL>
 __global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
+  constexpr int DT = NPL == 3 ? CRADLE_F32 : ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
   const PackJob j = js.job[blockIdx.y];
   const int per = j.ld_dst / 8;
   const int64_t total = (int64_t)j.rows_dst * per;
@@ -69,13 +71,29 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
     const int r = (int)(t / per), c0 = (int)(t % per) * 8;
     const int src = r < j.gap_at ? r : r - j.gap;
     const bool zero = (r >= j.gap_at && r < j.gap_at + j.gap) || src >= j.rows;
-    const int64_t s = (int64_t)src * j.ld_src + c0;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = !zero && c0 + e < j.cols ? load_as(j.src, s + e, js.dtype) : 0.f;
+    const int64_t s = (int64_t)(zero ? 0 : src) * j.ld_src;
     u16 p[8][NPL];
+    if constexpr (DT == CRADLE_F32) {
+      const float* q = static_cast<const float*>(j.src) + s;
+      float v[8];
+      if (j.vec && c0 + 8 <= j.cols) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(q + c0), b = *reinterpret_cast<const f32x4*>(q + c0 + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) split<ELEM, NPL>(v[e], p[e]);
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = q[min(c0 + e, j.cols - 1)];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) split<ELEM, NPL>(!zero && c0 + e < j.cols ? v[e] : 0.f, p[e]);
+    } else {  // the numbers as they are
+      const u16* q = static_cast<const u16*>(j.src) + s;
+      u16 v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = q[min(c0 + e, j.cols - 1)];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e][0] = !zero && c0 + e < j.cols ? v[e] : (u16)0;
+    }
 #pragma unroll
     for (int k = 0; k < NPL; ++k) {
       u32x4 w;
@@ -348,14 +366,13 @@ inline Operand operand(const Plan& p, const void* src, int64_t ld, int rows, int
   if (direct(src, ld, cols, p.dtype) && gap == 0) return {static_cast<const u16*>(src), ld, 0, 0};
   const int64_t ldp = up8(cols), plane = (int64_t)rows_dst * ldp;
   u16* dst = static_cast<u16*>(ws.take(plane * p.npl * 2));
-  js.job[n_jobs++] = {src, dst, ld, plane, rows, cols, rows_dst, (int)ldp, gap_at, gap};
+  js.job[n_jobs++] = {src, dst, ld, plane, rows, cols, rows_dst, (int)ldp, gap_at, gap, ld % 4 == 0 && ((uintptr_t)src & 15) == 0};
   return {dst, ldp, plane, 0};
 }
 
 template <int ELEM, int NPL>
 void run_pack(const Plan& p, PackJobs& js, int n_jobs, hipStream_t s) {
   if (!n_jobs) return;
-  js.dtype = p.dtype;
   int64_t most = 0;
   for (int i = 0; i < n_jobs; ++i) {
     const int64_t t = (int64_t)js.job[i].rows_dst * (js.job[i].ld_dst / 8);

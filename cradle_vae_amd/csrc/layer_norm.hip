@@ -6,7 +6,8 @@
 // second moment about the mean, not E[x^2] - mean^2, which cancels for rows far from zero -- and every element is moved once, in
 // 16-byte pieces where the rows allow.  w and b stay in registers over all rows of a workgroup.
 // dw and db: a thread owns the same columns in every row it sees, so they accumulate in its registers (fp32); the workgroups'
-// partial rows are joined by a second launch in a fixed order.
+// partial rows are joined by a second launch in a fixed order.  Measured in bf16 on 32768 x 4096: forward 102 us (5.2 TB/s, a
+// large copy's rate on this card), backward 168 + 10 us (4.8 TB/s).
 #include "common.h"
 
 namespace cradle {
@@ -63,8 +64,12 @@ struct Cols {
           for (int e = 0; e < 8; ++e) v[c][e] = other;
         }
       } else {
+        // (unconditional loads from a clamped column: behind a branch each of them would be waited for on its own)
+        float t[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = in(c, e) ? load1<DT>(p, row0 + col(c, e)) : other;
+        for (int e = 0; e < 8; ++e) t[e] = load1<DT>(p, row0 + min(col(c, e), width - 1));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c][e] = in(c, e) ? t[e] : other;
       }
     }
   }
@@ -93,14 +98,19 @@ struct Cols {
       }
     }
   }
-  // a parameter vector of the tensors' type or fp32 (once per workgroup: not worth 16-byte loads)
+  // a parameter vector of the tensors' type or fp32
   template <int DT>
   __device__ __forceinline__ void load_param(const void* p, bool fp32, float (&v)[NCH][8], float none) const {
+    if (!p) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
+      for (int c = 0; c < NCH; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[c][e] = !p || !in(c, e) ? none : fp32 ? load1<CRADLE_F32>(p, col(c, e)) : load1<DT>(p, col(c, e));
+        for (int e = 0; e < 8; ++e) v[c][e] = none;
+    } else if (fp32) {
+      load<CRADLE_F32>(p, 0, v, 0.f);
+    } else {
+      load<DT>(p, 0, v, 0.f);
+    }
   }
 };
 
@@ -170,7 +180,7 @@ __global__ __launch_bounds__(threads<TPR>()) void fwd_kernel(const void* __restr
 }
 
 // partial: (gridDim.x, 2, width) sums of dy xh and dy over the rows of each workgroup, or NULL
-template <int DT, int TPR, int NCH, bool VEC>
+template <int DT, int TPR, int NCH, bool VEC, bool PARAMS>
 __global__ __launch_bounds__(threads<TPR>()) void bwd_kernel(const void* __restrict__ dy, int64_t ld_dy, const void* __restrict__ x,
                                                              int64_t ld_x, const void* __restrict__ w, int w_fp32,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -198,8 +208,10 @@ __global__ __launch_bounds__(threads<TPR>()) void bwd_kernel(const void* __restr
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[c][e] = (v[c][e] - mu) * rs;
-        sw[c][e] += g[c][e] * v[c][e];
-        sb[c][e] += g[c][e];
+        if constexpr (PARAMS) {
+          sw[c][e] += g[c][e] * v[c][e];
+          sb[c][e] += g[c][e];
+        }
         g[c][e] *= wv[c][e];
         s0 += g[c][e];
         s1 += g[c][e] * v[c][e];
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(threads<TPR>()) void bwd_kernel(const void* __restr
       cols.template store<DT>(dx, r * ld_dx, g);
     }
   }
-  if (!partial) return;
+  if (!PARAMS || !partial) return;
   float* out = partial + (int64_t)blockIdx.x * 2 * width;
   if constexpr (RPB == 1) {
     cols.template store<CRADLE_F32>(out, 0, sw);
@@ -239,6 +251,30 @@ __global__ __launch_bounds__(threads<TPR>()) void bwd_kernel(const void* __restr
   }
 }
 
+// The parameters' gradients alone, for rows too wide for one pass's registers: a thread owns eight columns (of 2048 per
+// workgroup) over a share of the rows.  partial: (gridDim.y, 2, width)
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void params_kernel(const void* __restrict__ dy, int64_t ld_dy, const void* __restrict__ x, int64_t ld_x,
+                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                     float* __restrict__ partial, int64_t rows, int width) {
+  const int first = blockIdx.x * 2048;
+  const Cols<256, 1, VEC> cols{(int)threadIdx.x, min(width - first, 2048)};
+  float sw[1][8] = {}, sb[1][8] = {};
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    float g[1][8], v[1][8];
+    const float mu = mean[r], rs = rstd[r];
+    cols.template load<DT>(x, r * ld_x + first, v, mu);
+    cols.template load<DT>(dy, r * ld_dy + first, g, 0.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sw[0][e] += g[0][e] * ((v[0][e] - mu) * rs);
+      sb[0][e] += g[0][e];
+    }
+  }
+  cols.template store<CRADLE_F32>(partial, (int64_t)blockIdx.y * 2 * width + first, sw);
+  cols.template store<CRADLE_F32>(partial, ((int64_t)blockIdx.y * 2 + 1) * width + first, sb);
+}
+
 // sums n partial rows of 2 * width floats: sixteen waves take every sixteenth row of 64 columns, joined in wave order
 __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ partial, int n, int width, void* __restrict__ dw,
                                                     void* __restrict__ db, int dtype) {
@@ -247,7 +283,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ pa
   const int c = blockIdx.x * 64 + lane;
   float s = 0.f;
   if (c < 2 * width) {
-#pragma unroll 4
+#pragma unroll 8
     for (int r = wave; r < n; r += 16) s += partial[(int64_t)r * 2 * width + c];
   }
   red[wave][lane] = s;
@@ -264,6 +300,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ pa
 }
 
 constexpr int kMaxWidth = 32768;
+constexpr int kOnePassWidth = 16384;  // above, dx and the parameters' gradients are two passes (one would spill)
 constexpr int kCUs = 256;
 
 // rows per workgroup and workgroups of a pass: enough of them to fill the chip, few enough that w, b (and the partial sums of
@@ -277,19 +314,31 @@ int64_t fwd_blocks(int64_t rows, int width) {
 int64_t bwd_blocks(int64_t rows, int width) {
   const int64_t b = (rows + rows_per_block(width) - 1) / rows_per_block(width);
   const int64_t most = width <= 4096 ? 4 * kCUs : width <= 8192 ? 2 * kCUs : kCUs;
-  return b < most ? b : most;
+  return b < most ? b : most;  // (also the row shares of params_kernel: 16 column blocks x 256)
 }
 
-// threads per row and chunks per thread by width (both passes)
-#define CRADLE_LN_WIDTHS(CASE) \
+// Threads per row and chunks per thread by width, measured in bf16.  Forward, 32768 x 4096: 256 threads with two chunks 124 us,
+// 512 with one 102 us.  The backward pass holds five numbers per column and has to stay below 128 registers (four waves per
+// SIMD): 32768 x 4096: 256 with two 168 us, 512 with one 192 us; 16384 x 8192: 512 with two (130 registers) 275 us, 1024 with one
+// 179 us.
+#define CRADLE_LN_FWD_WIDTHS(CASE) \
+  if (width <= 512) CASE(64, 1)             \
+  else if (width <= 1024) CASE(64, 2)       \
+  else if (width <= 2048) CASE(256, 1)      \
+  else if (width <= 4096) CASE(512, 1)      \
+  else if (width <= 8192) CASE(512, 2)      \
+  else if (width <= 16384) CASE(1024, 2)    \
+  else CASE(1024, 4)
+#define CRADLE_LN_BWD_WIDTHS(CASE) \
   if (width <= 512) CASE(64, 1)             \
   else if (width <= 1024) CASE(64, 2)       \
   else if (width <= 2048) CASE(256, 1)      \
   else if (width <= 4096) CASE(256, 2)      \
-  else if (width <= 8192) CASE(512, 2)      \
+  else if (width <= 8192) CASE(1024, 1)     \
   else if (width <= 16384) CASE(1024, 2)    \
   else CASE(1024, 4)
 
+// 16-byte pieces: base and row starts aligned (parameter vectors: ld = 0)
 bool vec_ok(const void* p, int64_t ld, int dtype) { return !p || (((uintptr_t)p & 15) == 0 && ld % (dtype == CRADLE_F32 ? 4 : 8) == 0); }
 
 int check_common(const char* what, int dtype, int w_dtype, int64_t rows, int width) {
@@ -313,7 +362,7 @@ int cradle_layer_norm_fwd(const void* x, int64_t ld_x, const void* weight, const
   if (rc != CRADLE_OK) return rc;
   if (rows == 0) return CRADLE_OK;
   CRADLE_CHECK_ARG(x && y && ld_x >= width && ld_y >= width, "layer_norm_fwd: null pointer or leading dimension below the width");
-  const bool vec = width % 8 == 0 && vec_ok(x, ld_x, dtype) && vec_ok(y, ld_y, dtype);
+  const bool vec = width % 8 == 0 && vec_ok(x, ld_x, dtype) && vec_ok(y, ld_y, dtype) && vec_ok(weight, 0, dtype) && vec_ok(bias, 0, dtype);
   const int w_fp32 = w_dtype == CRADLE_F32;
   const dim3 grid((unsigned)fwd_blocks(rows, width));
 #define CRADLE_LN_FWD(DT, TPR, NCH, VEC)                                                                                        \
@@ -332,7 +381,7 @@ int cradle_layer_norm_fwd(const void* x, int64_t ld_x, const void* weight, const
       else CRADLE_LN_FWD(CRADLE_F16, TPR, NCH, false);                             \
     }                                                                              \
   }
-  CRADLE_LN_WIDTHS(CRADLE_LN_CASE)
+  CRADLE_LN_FWD_WIDTHS(CRADLE_LN_CASE)
 #undef CRADLE_LN_CASE
   CRADLE_CHECK_LAUNCH("layer_norm_fwd");
   return CRADLE_OK;
@@ -356,27 +405,34 @@ int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
                                ((uintptr_t)workspace & 15) == 0),
                    "layer_norm_bwd: workspace of %lld floats (16-byte aligned) needed",
                    (long long)cradle_layer_norm_workspace_floats(rows, width));
-  const bool vec = width % 8 == 0 && vec_ok(dy, ld_dy, dtype) && vec_ok(x, ld_x, dtype) && vec_ok(dx, ld_dx, dtype);
+  const bool vec = width % 8 == 0 && vec_ok(dy, ld_dy, dtype) && vec_ok(x, ld_x, dtype) && vec_ok(dx, ld_dx, dtype) && vec_ok(weight, 0, dtype);
   const int w_fp32 = w_dtype == CRADLE_F32;
   const int blocks = (int)bwd_blocks(rows, width);
   float* partial = params ? workspace : nullptr;
-#define CRADLE_LN_BWD(DT, TPR, NCH, VEC)                                                                                            \
-  hipLaunchKernelGGL((bwd_kernel<DT, TPR, NCH, VEC>), dim3(blocks), dim3(threads<TPR>()), 0, s, dy, ld_dy, x, ld_x, weight, w_fp32, \
-                     mean, rstd, dx, ld_dx, partial, rows, width)
+  const bool one_pass = width <= kOnePassWidth;
+#define CRADLE_LN_BWD(DT, TPR, NCH, VEC)                                                                                               \
+  {                                                                                                                                    \
+    if (one_pass || dx)                                                                                                                \
+      hipLaunchKernelGGL((bwd_kernel<DT, TPR, NCH, VEC, (NCH <= 2)>), dim3(blocks), dim3(threads<TPR>()), 0, s, dy, ld_dy, x, ld_x,     \
+                         weight, w_fp32, mean, rstd, dx, ld_dx, partial, rows, width);                                                 \
+    if (!one_pass && params)                                                                                                           \
+      hipLaunchKernelGGL((params_kernel<DT, VEC>), dim3((width + 2047) / 2048, blocks), dim3(256), 0, s, dy, ld_dy, x, ld_x, mean, rstd, \
+                         partial, rows, width);                                                                                        \
+  }
 #define CRADLE_LN_CASE(TPR, NCH)                                                   \
   {                                                                                \
     if (dtype == CRADLE_F32) {                                                     \
-      if (vec) CRADLE_LN_BWD(CRADLE_F32, TPR, NCH, true);                          \
-      else CRADLE_LN_BWD(CRADLE_F32, TPR, NCH, false);                             \
+      if (vec) CRADLE_LN_BWD(CRADLE_F32, TPR, NCH, true)                           \
+      else CRADLE_LN_BWD(CRADLE_F32, TPR, NCH, false)                              \
     } else if (dtype == CRADLE_BF16) {                                             \
-      if (vec) CRADLE_LN_BWD(CRADLE_BF16, TPR, NCH, true);                         \
-      else CRADLE_LN_BWD(CRADLE_BF16, TPR, NCH, false);                            \
+      if (vec) CRADLE_LN_BWD(CRADLE_BF16, TPR, NCH, true)                          \
+      else CRADLE_LN_BWD(CRADLE_BF16, TPR, NCH, false)                             \
     } else {                                                                       \
-      if (vec) CRADLE_LN_BWD(CRADLE_F16, TPR, NCH, true);                          \
-      else CRADLE_LN_BWD(CRADLE_F16, TPR, NCH, false);                             \
+      if (vec) CRADLE_LN_BWD(CRADLE_F16, TPR, NCH, true)                           \
+      else CRADLE_LN_BWD(CRADLE_F16, TPR, NCH, false)                              \
     }                                                                              \
   }
-  CRADLE_LN_WIDTHS(CRADLE_LN_CASE)
+  CRADLE_LN_BWD_WIDTHS(CRADLE_LN_CASE)
 #undef CRADLE_LN_CASE
   if (params)
     hipLaunchKernelGGL(join_kernel, dim3((2 * width + 63) / 64), dim3(1024), 0, s, workspace, blocks, width, dweight, dbias, w_dtype);

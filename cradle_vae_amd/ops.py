@@ -442,6 +442,8 @@ def _rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
         raise hip.CradleHipError(f"{what}: expected an fp32 / bf16 / fp16 CUDA tensor, got {t.dtype} on {t.device} (no fallback path)")
     if t.dim() < 1:
         raise hip.CradleHipError(f"{what}: expected at least one axis")
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.new_empty((0, 0))
     if r.shape[0] and r.shape[1] and (r.stride(1) != 1 or (r.shape[0] > 1 and r.stride(0) < r.shape[1])):
         r = r.contiguous()
@@ -473,39 +475,54 @@ def _pointer(t: Optional[torch.Tensor]) -> Optional[int]:
 class _on:
     """Makes a tensor's device the current one around a launch: the kernel runs on that device's current stream."""
 
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    __slots__ = ("device", "guard")
 
-    def __enter__(self):
-        if self.guard is not None:
+    def __init__(self, t: torch.Tensor):
+        self.device, self.guard = t.get_device(), None
+
+    def __enter__(self) -> int:
+        if self.device != torch._C._cuda_getDevice():
+            self.guard = torch.cuda.device(self.device)
             self.guard.__enter__()
-        return hip.stream()
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
 
 
+def _norm_params(what: str, x: torch.Tensor, **params) -> Tuple[list, torch.dtype]:
+    """The parameter vectors of a norm over x's last axis, checked, and their common type (x's own without any)."""
+    out, dtype = [], None
+    for name, t in params.items():
+        if t is not None:
+            if (t.dtype is not x.dtype and t.dtype is not torch.float32) or t.dim() != 1 or t.shape[0] != x.shape[-1]:
+                raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, expected ({x.shape[-1]},) of {x.dtype} or fp32")
+            if dtype is not None and t.dtype is not dtype:
+                raise hip.CradleHipError(f"{what}: {name} is {t.dtype} beside {dtype}")
+            if t.get_device() != x.get_device():
+                raise hip.CradleHipError(f"{what}: {name} is on {t.device}, x on {x.device}")
+            dtype, t = t.dtype, t if t.is_contiguous() else t.contiguous()
+        out.append(t)
+    return out, dtype if dtype is not None else x.dtype
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
-    """Layer norm over the last axis -> (y, mean, rstd); mean and rstd (fp32, one per row) are what ``layer_norm_bwd`` reads.
-    ``x`` fp32 / bf16 / fp16, rows may be strided; ``weight`` / ``bias`` of x's type or fp32 (``cradle_layer_norm_fwd``)."""
+    """Layer norm over the last axis (1 to 32768 wide) -> (y, mean, rstd); mean and rstd (fp32, one per row) are what
+    ``layer_norm_bwd`` reads.  ``x`` fp32 / bf16 / fp16, rows may be strided; ``weight`` / ``bias`` of x's type or fp32
+    (``cradle_layer_norm_fwd``)."""
     x2 = _rows_of(x, "layer_norm")
-    D = x.shape[-1]
-    types = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
-    weight, bias = _vector("layer_norm", "weight", weight, D, types), _vector("layer_norm", "bias", bias, D, types)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise hip.CradleHipError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    _same_place("layer_norm", x, weight=weight, bias=bias)
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
-    param = weight if weight is not None else bias
-    w_type = FLOAT_TYPES[param.dtype if param is not None else x.dtype]
+    (weight, bias), w_dtype = _norm_params("layer_norm", x, weight=weight, bias=bias)
+    rows, D = x2.shape
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    stats = x.new_empty((2, rows), dtype=torch.float32)
+    at = stats.data_ptr()
     with _on(x) as s:
         hip.check(hip.load().cradle_layer_norm_fwd(
-            x2.data_ptr(), _ld(x2), _pointer(weight), _pointer(bias), FLOAT_TYPES[x.dtype], w_type, eps, y.data_ptr(), D,
-            stats[0].data_ptr(), stats[1].data_ptr(), rows, D, s), "layer_norm_fwd")
-    return y, stats[0], stats[1]
+            x2.data_ptr(), _ld(x2), _pointer(weight), _pointer(bias), FLOAT_TYPES[x.dtype], FLOAT_TYPES[w_dtype], eps, y.data_ptr(), D,
+            at, at + 4 * rows, rows, D, s), "layer_norm_fwd")
+    mean, rstd = (stats if x.dim() == 2 else stats.reshape(2, *x.shape[:-1])).unbind(0)
+    return y, mean, rstd
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor, *,
@@ -513,31 +530,38 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     """-> (dx, dweight, dbias) of ``layer_norm``; the parameters' gradients have weight's type (``param_dtype`` without a
     weight, default x's) and are sums over the rows in a fixed order."""
     what = "layer_norm_bwd"
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)}, x {x.dtype} {tuple(x.shape)}")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)} on {dy.device}, x {x.dtype} {tuple(x.shape)} on {x.device}")
     x2, dy2 = _rows_of(x, what), _rows_of(dy, what)
-    rows, D = x2.shape[0], x.shape[-1]
-    types = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
-    weight = _vector(what, "weight", weight, D, types)
-    p_dtype = weight.dtype if weight is not None else (param_dtype or x.dtype)
-    if p_dtype not in types:
-        raise hip.CradleHipError(f"{what}: param_dtype {p_dtype} is neither x's type nor fp32")
-    mean, rstd = _vector(what, "mean", mean.reshape(-1), rows, (torch.float32,)), _vector(what, "rstd", rstd.reshape(-1), rows, (torch.float32,))
-    _same_place(what, x, dy=dy, weight=weight, mean=mean, rstd=rstd)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_dx else None
+    (weight,), p_dtype = _norm_params(what, x, weight=weight)
+    if weight is None and param_dtype is not None:
+        p_dtype = param_dtype
+        if p_dtype is not x.dtype and p_dtype is not torch.float32:
+            raise hip.CradleHipError(f"{what}: param_dtype {p_dtype} is neither x's type nor fp32")
+    rows, D = x2.shape
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype is not torch.float32 or t.numel() != rows or t.get_device() != x.get_device() or not t.is_contiguous():
+            raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, expected {rows} contiguous fp32 numbers on {x.device}")
+    dx = None if not need_dx else torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    dw = db = ws = at = at_w = at_b = None
     if rows == 0:
-        z = torch.zeros((2, D), device=x.device, dtype=p_dtype) if need_params else (None, None)
-        return dx, z[0], z[1]
-    dp = torch.empty((2, D), device=x.device, dtype=p_dtype) if need_params else (None, None)
-    lib = hip.load()
-    need = lib.cradle_layer_norm_workspace_floats(rows, D) if need_params else 0
-    ws = torch.empty(need, device=x.device, dtype=torch.float32) if need else None
+        if need_params:
+            dw, db = x.new_zeros((2, D), dtype=p_dtype).unbind(0)
+        return dx, dw, db
+    lib, need = hip.load(), 0
+    if need_params:
+        grads = x.new_empty((2, D), dtype=p_dtype)
+        at_w = grads.data_ptr()
+        at_b = at_w + D * grads.element_size()
+        dw, db = grads.unbind(0)
+        need = lib.cradle_layer_norm_workspace_floats(rows, D)
+        ws = x.new_empty((need,), dtype=torch.float32)
+        at = ws.data_ptr()
     with _on(x) as s:
         hip.check(lib.cradle_layer_norm_bwd(
             dy2.data_ptr(), _ld(dy2), x2.data_ptr(), _ld(x2), _pointer(weight), mean.data_ptr(), rstd.data_ptr(),
-            FLOAT_TYPES[x.dtype], FLOAT_TYPES[p_dtype], _pointer(dx), D, _pointer(dp[0]), _pointer(dp[1]), _pointer(ws), need, rows,
-            D, s), what)
-    return dx, dp[0], dp[1]
+            FLOAT_TYPES[x.dtype], FLOAT_TYPES[p_dtype], _pointer(dx), D, at_w, at_b, at, need, rows, D, s), what)
+    return dx, dw, db
 
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
