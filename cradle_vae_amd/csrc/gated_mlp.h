@@ -7,7 +7,8 @@
 //
 // Numbers: bf16 / fp16 tensors multiply as they are; fp32 tensors as three bf16 planes (six products, fp32's accuracy at
 // 2.6x the rate of the fp32 matrix instruction).  Sums, pre-activations and biases are fp32.  h and [dg | du] are inputs of a
-// matrix product and so are rounded once to the operand's type: an error of the size of the result's own last rounding.
+// matrix product and so are rounded once to the operand's type, an error of the size of the result's own last rounding; small
+// blocks, whose few numbers would not average it out and which are bound by latency, keep them in two planes instead.
 // The saved pre-activations stay fp32 (rounded to bf16 they would put two more roundings into every gradient).
 // A handful of rows (inference of single cells) take kernels that read the weights once, coalesced, with fp32 arithmetic.
 #pragma once
@@ -324,10 +325,14 @@ inline int esize(int dtype) { return dtype == CRADLE_F32 ? 4 : 2; }
 constexpr int kFewRows = 4;   // rows up to which the weights' reading bounds the block (measured beside few_rows)
 constexpr int kCUs = 256;
 
+// Below this many products per projection (2^28: under 2 us of the matrix cores) a block's time is its launches, and the second
+// plane of h and [dg | du] costs nothing that shows; above, it would cost a third of the forward and most of the backward pass again.
+constexpr int64_t kSmallWork = 1LL << 28;
+
 struct Plan {
   int M, K, F, O, Fp;
   int dtype, elem, npl;  // planes of the tensors' operands
-  int nph;               // planes of h and [dg | du]
+  int nph;               // planes of h and [dg | du]: twice a 16-bit tensor's bits while that is free
 };
 
 inline Plan plan_of(const cradle_gated_mlp_desc* d) {
@@ -340,7 +345,7 @@ inline Plan plan_of(const cradle_gated_mlp_desc* d) {
   p.dtype = d->dtype;
   p.elem = d->dtype == CRADLE_F16 ? F16 : BF16;
   p.npl = d->dtype == CRADLE_F32 ? 3 : 1;
-  p.nph = p.npl;
+  p.nph = p.npl == 1 && (int64_t)p.M * p.F * (p.K + p.O) < kSmallWork ? 2 : p.npl;
   return p;
 }
 
@@ -383,13 +388,13 @@ void run_pack(const Plan& p, PackJobs& js, int n_jobs, hipStream_t s) {
   hipLaunchKernelGGL((pack_kernel<ELEM, NPL>), grid, dim3(256), 0, s, js);
 }
 
-// Two tiles per operand format.  Large: 256 x 256 (three planes: 256 x 128, to fit the LDS), eight waves, one workgroup per CU.
-// Small: 128 x 128 (three planes: 128 x 64), four waves, two workgroups per CU.
+// Two tiles per operand format.  Large: 256 x 256 (more than one plane: 256 x 128, to fit the LDS), eight waves, one workgroup per
+// CU.  Small: 128 x 128 (more than one plane: 128 x 64), four waves, two workgroups per CU.
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
 struct Tiles {
-  static constexpr bool ONE = NPA == 1 && NPB == 1;
-  using Large = Tile<ELEM, NPA, NPB, 256, ONE ? 256 : 128, ONE ? 64 : 32, 2, ONE ? 2 : 4, ONE ? 4 : 2, AK, BK>;
-  using Small = Tile<ELEM, NPA, NPB, 128, ONE ? 128 : 64, ONE ? 64 : 32, 2, ONE ? 2 : 4, ONE ? 2 : 1, AK, BK>;
+  static constexpr bool ONE = NPA == 1 && NPB == 1, THREE = NPA == 3;
+  using Large = Tile<ELEM, NPA, NPB, 256, ONE ? 256 : 128, ONE ? 64 : 32, ONE || THREE ? 2 : 3, ONE ? 2 : 4, ONE ? 4 : 2, AK, BK>;
+  using Small = Tile<ELEM, NPA, NPB, 128, ONE ? 128 : 64, THREE ? 32 : 64, 2, ONE ? 2 : 4, ONE ? 2 : 1, AK, BK>;
 };
 
 template <class T, class Epi>
@@ -467,7 +472,7 @@ inline Args args_of(const Operand& A, const Operand& B, int M, int N, int K) {
 }
 
 // ---- forward: workspace = packed x, W_in, W_out | h when it is not saved | partial sums
-template <int ELEM, int NPL>
+template <int ELEM, int NPL, int NPH>
 int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
   Bump ws{static_cast<char*>(workspace)};
   PackJobs js{};
@@ -477,16 +482,16 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, ws, js, n);
   const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp;
-  u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * p.nph * 2));
-  float* partial = static_cast<float*>(ws.take(partial_floats<ELEM, NPL, NPL, true, true>(p.M, p.O, p.Fp) * 4));
+  u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * NPH * 2));
+  float* partial = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, true>(p.M, p.O, p.Fp) * 4));
   if (!run) return ws.off;
   run_pack<ELEM, NPL>(p, js, n, s);
   Args a = args_of(x, w_in, p.M, p.F, p.K);
   a.up_row = p.Fp;
   product<ELEM, NPL, NPL, true, true>(
-      a, GateEpi<ELEM, NPL>{d->act, p.F, p.Fp, p.dtype, d->b_in, h, h_plane, static_cast<float*>(d->saved_gu)}, p.F, s);
+      a, GateEpi<ELEM, NPH>{d->act, p.F, p.Fp, p.dtype, d->b_in, h, h_plane, static_cast<float*>(d->saved_gu)}, p.F, s);
   const Operand hop{h, p.Fp, h_plane, 0};
-  product_out<ELEM, NPL, NPL, true, true>(
+  product_out<ELEM, NPH, NPL, true, true>(
       args_of(hop, w_out, p.M, p.O, p.Fp),
       OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, vec_ok(d->y, d->ld_y, p.dtype)}, partial, s);
   return ws.off;
@@ -499,7 +504,7 @@ inline int colsum_rows(int rows) {
 }
 
 // ---- backward: workspace = packed x, W_in, W_out, dy | [dg | du] | partial sums | column-sum partials
-template <int ELEM, int NPL>
+template <int ELEM, int NPL, int NPH>
 int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
   Bump ws{static_cast<char*>(workspace)};
   PackJobs js{};
@@ -510,10 +515,10 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
   const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp, d_plane = 2 * h_plane;
-  u16* dgu = static_cast<u16*>(ws.take(d_plane * p.nph * 2));
-  int64_t pf = partial_floats<ELEM, NPL, NPL, true, false>(p.M, p.K, 2 * p.Fp);
-  const int64_t pf1 = partial_floats<ELEM, NPL, NPL, false, false>(2 * p.Fp, p.K, p.M);
-  const int64_t pf2 = partial_floats<ELEM, NPL, NPL, false, false>(p.O, p.F, p.M);
+  u16* dgu = static_cast<u16*>(ws.take(d_plane * NPH * 2));
+  int64_t pf = partial_floats<ELEM, NPH, NPL, true, false>(p.M, p.K, 2 * p.Fp);
+  const int64_t pf1 = partial_floats<ELEM, NPH, NPL, false, false>(2 * p.Fp, p.K, p.M);
+  const int64_t pf2 = partial_floats<ELEM, NPL, NPH, false, false>(p.O, p.F, p.M);
   pf = pf > pf1 ? pf : pf1;
   pf = pf > pf2 ? pf : pf2;
   float* partial = static_cast<float*>(ws.take(pf * 4));
@@ -528,7 +533,7 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   using TT = Tiles<ELEM, NPL, NPL, true, false>;
   const bool large = use_large<typename TT::Large, typename TT::Small>(a, p.F, false);
   product<ELEM, NPL, NPL, true, false>(
-      a, GateBwdEpi<ELEM, NPL>{d->act, p.F, p.Fp, static_cast<const float*>(d->saved_gu), dgu, d_plane, d->db_in ? sums : nullptr}, p.F, s);
+      a, GateBwdEpi<ELEM, NPH>{d->act, p.F, p.Fp, static_cast<const float*>(d->saved_gu), dgu, d_plane, d->db_in ? sums : nullptr}, p.F, s);
   if (d->db_in) {
     const int used = large ? (p.M + 255) / 256 * TT::Large::WAVES_M : (p.M + 127) / 128 * TT::Small::WAVES_M;
     hipLaunchKernelGGL(colsum_join_kernel, dim3((2 * p.F + 63) / 64), dim3(1024), 0, s, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
@@ -543,20 +548,19 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g) {
     return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, vec_ok(q, ld, p.dtype)};
   };
-  if (d->dx) product_out<ELEM, NPL, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0), partial, s);
-  if (d->dw_in) product_out<ELEM, NPL, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap), partial, s);
-  if (d->dw_out) product_out<ELEM, NPL, NPL, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0), partial, s);
+  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0), partial, s);
+  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap), partial, s);
+  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0), partial, s);
   return ws.off;
 }
 
 // Both passes per type, each in a source of its own (gated_mlp_{f32,bf16,f16}.hip).  run = false: only the workspace is sized.
-#define CRADLE_GATED_TYPE(NAME) \
-  int64_t forward_##NAME(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);  \
-  int64_t backward_##NAME(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
-CRADLE_GATED_TYPE(f32)
-CRADLE_GATED_TYPE(bf16)
-CRADLE_GATED_TYPE(f16)
-#undef CRADLE_GATED_TYPE
+int64_t forward_f32(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+int64_t forward_bf16(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+int64_t forward_f16(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+int64_t backward_f32(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+int64_t backward_bf16(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
+int64_t backward_f16(const cradle_gated_mlp_desc*, const Plan&, void* workspace, hipStream_t, bool run);
 
 }  // namespace gated
 }  // namespace cradle

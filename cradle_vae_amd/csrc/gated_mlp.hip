@@ -151,9 +151,12 @@ using namespace cradle::gated;
 
 extern "C" {
 
-int64_t cradle_gated_mlp_saved_bytes(int rows, int hidden, int dtype, int64_t* h_bytes) {
-  const int64_t n = (int64_t)rows * up8(hidden);
-  if (h_bytes) *h_bytes = n * 2 * (dtype == CRADLE_F32 ? 3 : 1);
+int64_t cradle_gated_mlp_saved_bytes(int rows, int width, int hidden, int out_width, int dtype, int64_t* h_bytes) {
+  cradle_gated_mlp_desc d{};
+  d.rows = rows, d.width = width, d.hidden = hidden, d.out_width = out_width, d.dtype = dtype;
+  const Plan p = plan_of(&d);
+  const int64_t n = (int64_t)rows * p.Fp;
+  if (h_bytes) *h_bytes = n * 2 * p.nph;
   return n * 2 * 4;
 }
 

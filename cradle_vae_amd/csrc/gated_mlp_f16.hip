@@ -1,13 +1,13 @@
-// The gated feed-forward block's products for fp16 tensors.
+// The gated feed-forward block's products for fp16 tensors: h and [dg | du] as the tensors' numbers or in two planes.
 #include "gated_mlp.h"
 
 namespace cradle {
 namespace gated {
 int64_t forward_f16(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
-  return forward<F16, 1>(d, p, workspace, s, run);
+  return (p.nph == 2 ? forward<F16, 1, 2> : forward<F16, 1, 1>)(d, p, workspace, s, run);
 }
 int64_t backward_f16(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
-  return backward<F16, 1>(d, p, workspace, s, run);
+  return (p.nph == 2 ? backward<F16, 1, 2> : backward<F16, 1, 1>)(d, p, workspace, s, run);
 }
 }  // namespace gated
 }  // namespace cradle

@@ -101,7 +101,7 @@ PROTOTYPES = {
         [ctypes.c_void_p, i64, ctypes.c_void_p, i64, ctypes.c_void_p, c_float_p, c_float_p, i32, i32, ctypes.c_void_p, i64,
          ctypes.c_void_p, ctypes.c_void_p, c_float_p, i64, i64, i32, c_stream],
     ),
-    "cradle_gated_mlp_saved_bytes": (i64, [i32, i32, i32, ctypes.POINTER(i64)]),
+    "cradle_gated_mlp_saved_bytes": (i64, [i32, i32, i32, i32, i32, ctypes.POINTER(i64)]),
     "cradle_gated_mlp_workspace_bytes": (i64, [ctypes.c_void_p, i32]),
     "cradle_gated_mlp_fwd": (i32, [ctypes.c_void_p, c_stream]),
     "cradle_gated_mlp_bwd": (i32, [ctypes.c_void_p, c_stream]),

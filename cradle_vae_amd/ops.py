@@ -620,7 +620,7 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     lib, saved = hip.load(), None
     if save:
         hb = ctypes.c_int64()
-        gb = lib.cradle_gated_mlp_saved_bytes(M, F, d.dtype, ctypes.byref(hb))
+        gb = lib.cradle_gated_mlp_saved_bytes(M, d.width, F, O, d.dtype, ctypes.byref(hb))
         saved = (torch.empty(gb // 4, device=x.device, dtype=torch.float32), torch.empty(hb.value // 2, device=x.device, dtype=torch.int16))
         if M:
             d.saved_gu, d.saved_h = saved[0].data_ptr(), saved[1].data_ptr()
@@ -644,7 +644,7 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
         raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)}, expected {x.dtype} {(*x.shape[:-1], O)}")
     _same_place(what, x, dy=dy, saved_gu=saved[0], saved_h=saved[1])
     lib, hb = hip.load(), ctypes.c_int64()
-    gb = lib.cradle_gated_mlp_saved_bytes(M, F, d.dtype, ctypes.byref(hb))
+    gb = lib.cradle_gated_mlp_saved_bytes(M, d.width, F, O, d.dtype, ctypes.byref(hb))
     if saved[0].numel() * 4 != gb or saved[1].numel() * 2 != hb.value:
         raise hip.CradleHipError(f"{what}: the saved buffers do not belong to a block of these sizes")
     make = torch.empty if M else torch.zeros

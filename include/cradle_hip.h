@@ -442,7 +442,8 @@ int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
  * Training: saved_gu and saved_h (cradle_gated_mlp_saved_bytes) receive what the backward pass reads; NULL for inference.
  * cradle_gated_mlp_bwd: from dy (rows, out_width) and the saved buffers, dx (rows, width; NULL = not needed), dw_in, dw_out
  * (contiguous, NULL = not needed), db_in, db_out (NULL = not needed).  The residual's gradient is dy.
- * h and [dg | du] are rounded to the tensors' type where they enter a matrix product (fp32: to 24 bits).  fp32 inputs of
+ * h and [dg | du] are rounded to the tensors' type where they enter a matrix product (fp32: to 24 bits; 16-bit types of small
+ * blocks, rows * hidden * (width + out_width) < 2^28: to twice their bits).  fp32 inputs of
  * magnitude above 3.39e38 count as infinite.  workspace: cradle_gated_mlp_workspace_bytes(desc, backward) bytes, 16-byte aligned;
  * only the sizes, types, pointers' alignment and which pointers are NULL are read for it.
  * hidden * ld_w_in < 2^30, widths <= 2^20, leading dimensions < 2^22. */
@@ -466,7 +467,7 @@ typedef struct cradle_gated_mlp_desc {
   void* workspace; int64_t workspace_bytes;
 } cradle_gated_mlp_desc;
 /* bytes of saved_gu (returned) and of saved_h (*h_bytes) */
-int64_t cradle_gated_mlp_saved_bytes(int rows, int hidden, int dtype, int64_t* h_bytes);
+int64_t cradle_gated_mlp_saved_bytes(int rows, int width, int hidden, int out_width, int dtype, int64_t* h_bytes);
 int64_t cradle_gated_mlp_workspace_bytes(const cradle_gated_mlp_desc* desc, int backward_pass);
 int cradle_gated_mlp_fwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stream);
 int cradle_gated_mlp_bwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stream);
