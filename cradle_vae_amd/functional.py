@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -209,3 +210,60 @@ class _OneHotLinear(torch.autograd.Function):
 
 def onehot_linear(mask: torch.Tensor, W: torch.Tensor, b: torch.Tensor, t0: int = 0) -> torch.Tensor:
     return _OneHotLinear.apply(mask, W, b, t0)
+
+
+# ---------------------------------------------------------------------------------------------
+# normalised, gated hidden layers (no counterpart in the reference's LeakyReLU MLPs)
+# ---------------------------------------------------------------------------------------------
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.layer_norm_bwd(dy, x, weight, mean, rstd, need_dx=need[0], need_params=need[1] or need[2],
+                                        param_dtype=ctx.bias_dtype)
+        return dx, dw if need[1] else None, db if need[2] else None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last axis with its gradients (``ops.layer_norm``): fp32 / bf16 / fp16, parameters of x's type or
+    fp32."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return ops.layer_norm(x, weight, bias, eps)[0]
+
+
+class _GatedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, b_in, b_out, residual, act):
+        y, saved = ops.gated_mlp(x, w_in, w_out, b_in, b_out, act=act, residual=residual, save=True)
+        ctx.save_for_backward(x, w_in, w_out, *saved)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_in, w_out, *saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw_in, dw_out, db_in, db_out = ops.gated_mlp_bwd(dy, x, w_in, w_out, saved, act=ctx.act, bias=need[3] or need[4],
+                                                             need=need[:3])
+        return dx, dw_in, dw_out, db_in if need[3] else None, db_out if need[4] else None, dy if need[5] else None, None
+
+
+def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
+              b_out: Optional[torch.Tensor] = None, act: str = "silu", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gated feed-forward block with its gradients: (act(g) * u) w_out^T + b_out (+ residual), [g | u] = x w_in^T + b_in
+    (``ops.gated_mlp``).  Without anything to differentiate nothing is saved."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out, residual)):
+        return _GatedMLP.apply(x, w_in, w_out, b_in, b_out, residual, act)
+    return ops.gated_mlp(x, w_in, w_out, b_in, b_out, act=act, residual=residual)

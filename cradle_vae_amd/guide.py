@@ -63,6 +63,7 @@ class cradle_vae_CorrelatedNormalGuide(nn.Module):
         mask_init_logits: float = 0,
         gs_temperature: float = 1,
         mean_field_encoder: bool = False,
+        mlp_block: str = "residual",
     ):
         super().__init__()
         if mean_field_encoder:
@@ -78,7 +79,8 @@ class cradle_vae_CorrelatedNormalGuide(nn.Module):
         self.param_dict = nn.ParameterDict()
         self.param_dict["q_mask_logits"] = nn.Parameter(mask_init_logits * torch.ones((n_treatments, n_latent)))
         self.embedding_encoder = get_likelihood_mlp(
-            "normal", n_latent + n_treatments, n_latent, embedding_encoder_n_layers, embedding_encoder_n_hidden)
+            "normal", n_latent + n_treatments, n_latent, embedding_encoder_n_layers, embedding_encoder_n_hidden,
+            block=mlp_block)
         # kept for state-dict compatibility (correlated_normal_guide.py:64) while it is small; the HIP path never
         # multiplies by it (the one-hot block of the first layer is a column lookup), and at 10 k treatments it
         # would be 400 MB of identity matrix: beyond MAX_ONE_HOT_BUFFER treatments the key is dropped on load
@@ -87,9 +89,10 @@ class cradle_vae_CorrelatedNormalGuide(nn.Module):
         self.normalization_module = LogStandardizationModule(x_normalization_stats)
         self.register_buffer("qc_encoder_input", torch.ones((n_qc, n_latent)))
         self.qc_encoder = get_likelihood_mlp(
-            "normal", n_latent, n_latent, embedding_encoder_n_layers, embedding_encoder_n_hidden)
+            "normal", n_latent, n_latent, embedding_encoder_n_layers, embedding_encoder_n_hidden,
+            block=mlp_block)
         self.z_basal_encoder = get_likelihood_mlp(
-            "normal", n_phenos + 2 * n_latent, n_latent, basal_encoder_n_layers, basal_encoder_n_hidden)
+            "normal", n_phenos + 2 * n_latent, n_latent, basal_encoder_n_layers, basal_encoder_n_hidden, block=mlp_block)
         self.register_buffer("gs_temperature", gs_temperature * torch.ones((1,)))
         self.var_eps = 1e-4
         # matmul(D, .) runs through the non-zero dosages of each cell (<= this many; a row with more raises the
@@ -267,7 +270,7 @@ class cradle_vae_CorrelatedNormalGuide(nn.Module):
         enc = self.embedding_encoder
         lins = enc.mlp.linears()
         h = F_hip.onehot_linear(mask, lins[0].weight, lins[0].bias, t0)
-        return enc.forward_from_hidden(h, first_layer_done=True)
+        return enc.forward_from_hidden(h)
 
     def dosage_product(self, D: torch.Tensor, table: torch.Tensor, P: int) -> torch.Tensor:
         """torch.matmul(D, table) for dosages D (N, T) and table (P, T, L) (correlated_normal_guide.py:186-188)

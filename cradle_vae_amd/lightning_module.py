@@ -18,6 +18,8 @@ from typing import Dict, Optional
 import torch
 import torch.nn as nn
 
+from .optim import OPTIMIZERS, make_optimizer
+
 try:  # pragma: no cover - pytorch_lightning is absent from the build image
     import pytorch_lightning as pl
 
@@ -69,8 +71,12 @@ class PerturbationLightningModule(_Base):
         predictor: Optional[nn.Module] = None,
         x_var_info=None,
         use_scheduler=False,
+        optimizer: str = "adam",
     ):
         super().__init__()
+        if optimizer not in OPTIMIZERS:
+            raise ValueError(f"optimizer={optimizer!r}: expected one of {OPTIMIZERS}")
+        self.optimizer_name = optimizer
         self.loss_module = loss_module
         self.lr = lr
         self.weight_decay = weight_decay
@@ -122,8 +128,8 @@ class PerturbationLightningModule(_Base):
         return loss
 
     def configure_optimizers(self):
-        """:147-164."""
-        optimizer = torch.optim.Adam(self.parameters(), lr=self.lr, weight_decay=self.weight_decay)
+        """:147-164; ``optimizer: muon`` (lightning_module_kwargs) is this build's own (optim.Muon)."""
+        optimizer = make_optimizer(self.optimizer_name, self, self.lr, self.weight_decay)
         if self.use_scheduler:
             optimizer = torch.optim.SGD(self.parameters(), lr=self.lr, weight_decay=self.weight_decay, momentum=0.9)
             scheduler = torch.optim.lr_scheduler.CyclicLR(

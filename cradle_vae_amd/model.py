@@ -23,6 +23,7 @@ class cradle_vae_Model(torch.nn.Module):
         decoder_n_layers: int,
         decoder_n_hidden: int,
         sum_mode: bool = True,
+        mlp_block: str = "residual",
     ):
         super().__init__()
         self.n_latent = n_latent
@@ -49,6 +50,7 @@ class cradle_vae_Model(torch.nn.Module):
             n_output=n_phenos,
             n_layers=decoder_n_layers + 1,
             n_hidden=decoder_n_hidden,
+            block=mlp_block,
         )
 
     def get_var_keys(self) -> List[str]:

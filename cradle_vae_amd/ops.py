@@ -670,6 +670,8 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)
 def _ns_bound(coeffs, steps: int) -> float:
     """Largest magnitude that s and b s^2 + c s^4 take over the iteration s <- a s + b s^3 + c s^5 from any s in [0, 1]."""
     a, b, c = (float(v) for v in coeffs)
+    if not all(abs(v) < float("inf") for v in (a, b, c)):
+        return float("inf")
     s, most = torch.linspace(0, 1, 4097, dtype=torch.float64), 1.0
     for _ in range(steps):
         q = b * s * s + c * s ** 4
@@ -689,8 +691,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float 
     what = "orthogonalize"
     if not g.is_cuda or g.dtype not in FLOAT_TYPES or g.dim() < 2:
         raise hip.CradleHipError(f"{what}: expected (..., m, n) fp32 / bf16 / fp16 on the GPU, got {g.dtype} {tuple(g.shape)} on {g.device}")
-    if not 1 <= int(steps) <= 64:
-        raise hip.CradleHipError(f"{what}: steps={steps} (1..64)")
+    if not 1 <= int(steps) <= 64 or not 0 <= eps < float("inf"):
+        raise hip.CradleHipError(f"{what}: steps={steps} (1..64), eps={eps}")
     coeffs = tuple(float(v) for v in coeffs)
     if len(coeffs) != 3 or not _ns_bound(coeffs, int(steps)) < 8:
         raise hip.CradleHipError(f"{what}: the iteration with coefficients {coeffs} does not stay within (-8, 8)")

@@ -26,7 +26,7 @@ OUT_KEYS = ["loss", "loss_term_reconstruction", "loss_term_mask", "loss_term_E",
 def unsupported_reason(lm):
     """None when the fused step runs this loss module, else what keeps it on the modular path (one sentence)."""
     from .guide import cradle_vae_CorrelatedNormalGuide
-    from .mlp import LibraryGammaPoissonSharedConcentrationResidualMLP
+    from .mlp import LibraryGammaPoissonSharedConcentrationResidualMLP, ResidualMLP
     from .model import cradle_vae_Model
 
     m, g = lm.model, lm.guide
@@ -36,6 +36,8 @@ def unsupported_reason(lm):
         return "sum_mode=True"
     if not isinstance(m.decoder, LibraryGammaPoissonSharedConcentrationResidualMLP):
         return f"likelihood {getattr(m, 'likelihood_key', '?')!r} (it implements library_nb)"
+    if not all(isinstance(e.mlp, ResidualMLP) for e in (m.decoder, g.embedding_encoder, g.qc_encoder, g.z_basal_encoder)):
+        return "mlp_block='gated'"
     if m.n_phenos < 4:
         return f"n_phenos={m.n_phenos} < 4"
     if not next(lm.parameters()).is_cuda:

@@ -14,16 +14,18 @@ import os
 import torch
 
 from . import parallel
+from .optim import make_optimizer
 
 
 class TrainStep:
     def __init__(self, loss_module, lr: float, weight_decay: float = 1e-6,
-                 gradient_clip_norm: Optional[float] = 100.0, world_size: int = 1, seed: int = 0):
+                 gradient_clip_norm: Optional[float] = 100.0, world_size: int = 1, seed: int = 0, optimizer: str = "adam"):
         self.lm = loss_module
         self.world_size = world_size
         self.clip = gradient_clip_norm
         self.params = [p for p in loss_module.parameters() if p.requires_grad]
-        self.optimizer = torch.optim.Adam(self.params, lr=lr, weight_decay=weight_decay)
+        self.optimizer_name = optimizer
+        self.optimizer = make_optimizer(optimizer, loss_module, lr, weight_decay)
         self.device = self.params[0].device
         # plated draws (mask, E, qc_E) must agree across ranks, local draws (z_basal) must not:
         # two generators, the first seeded identically everywhere
@@ -36,7 +38,12 @@ class TrainStep:
         self.fused = None
         # "device": the fused step draws its own noise (Philox, one launch); "torch": torch generators (4 launches)
         self.rng = os.environ.get("CRADLE_STEP_RNG", "device")
-        if loss_module._use_fused(None):
+        fused = loss_module._use_fused(None)
+        if fused and optimizer != "adam":
+            # the fused step's loss and gradients through its autograd node, the update by the optimiser (below)
+            self.impl = "fused+" + optimizer
+            loss_module._fused_step().defer_flag_check = world_size > 1  # (ranks raise together: check_flags)
+        elif fused:
             from . import hip
 
             self.fused = loss_module._fused_step()
@@ -224,6 +231,8 @@ class TrainStep:
         fused step's own check.  Collective for N > 1: every rank must call it at the same point (the step does so
         on its first training step and every 256th; trainer.fit at the end of every epoch and after validation)."""
         if self.fused is None:
+            if self.impl.startswith("fused+") and self.lm._fused_step().out is not None:
+                self._refuse_rejected_batch()
             return
         if self.world_size == 1:
             self.fused.check_flags()
@@ -244,6 +253,19 @@ class TrainStep:
                 f"rank {self.group_rank}: " + (mine or "another rank's step rejected its input") +
                 f"; {int(t[1])} parameter update(s) were skipped on all {self.world_size} ranks")
 
+    def _refuse_rejected_batch(self):
+        """The fused step of an optimiser other than Adam: no kernel skips the update of a rejected batch, so every step's
+        flags are looked at before it (one sync), on all ranks together."""
+        fused = self.lm._fused_step()
+        t = ((fused.flags != 0) | (fused.out[7] > 0)).float()
+        if self.world_size > 1:
+            parallel._all_reduce(t, op=torch.distributed.ReduceOp.MAX)
+        if float(t) > 0:
+            from . import hip
+
+            fused.check_flags()
+            raise hip.CradleHipError("another rank's step rejected its input; no parameter was updated")
+
     def __call__(self, batch: Dict[str, torch.Tensor], n_particles: int) -> torch.Tensor:
         if self.fused is not None:
             loss = self._fused_call(batch, n_particles)
@@ -260,6 +282,8 @@ class TrainStep:
             qc_obs_counts=batch["qc_obs_counts"], cfX=batch["cfX"],
             condition_values={"library_size": batch["library_size"]}, n_particles=n_particles, noise=noise,
             cf_noise=cf_noise)
+        if self.impl.startswith("fused+"):
+            self._refuse_rejected_batch()
         loss.backward()
         self.allreduce_grads()
         if self.clip is not None:
@@ -294,7 +318,8 @@ def fit(module, train_loader, val_loader=None, *, max_epochs: int = 1, max_steps
     if kmax and hasattr(module.loss_module, "max_dosages_per_cell"):
         module.loss_module.max_dosages_per_cell = max(kmax)
     stepper = TrainStep(module.loss_module, lr=module.lr, weight_decay=module.weight_decay,
-                        gradient_clip_norm=gradient_clip_val, world_size=world, seed=seed)
+                        gradient_clip_norm=gradient_clip_val, world_size=world, seed=seed,
+                        optimizer=getattr(module, "optimizer_name", "adam"))
     history, steps = [], 0
     for epoch in range(max_epochs):
         module.train()

@@ -153,3 +153,10 @@ def test_repeats_bit_for_bit():
         now = (y, *ops.gated_mlp_bwd(dy, x, w_in, w_out, saved, bias=True))
         assert first is None or all(torch.equal(p, q) for p, q in zip(first, now))
         first = now
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [True, False])
+def test_blocks_too_large_for_a_second_plane(dtype, bias):
+    # rows * hidden * (width + out) >= 2^28: h and [dg | du] in the tensors' type; no extent a multiple of a tile
+    _check(*_inputs(700, 633, 611, 592, dtype, bias=bias), act="gelu" if bias else "silu")
