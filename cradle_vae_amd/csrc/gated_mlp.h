@@ -109,12 +109,23 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
 // epilogues
 // ---------------------------------------------------------------------------------------------------------------
 struct NoState {};
+// a vector's four numbers at n (zero beyond its end, or without it)
+struct Four {
+  f32x4 v, w;
+};
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, int n, int dtype) {
+  f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) v[e] = load_as(p, i + e, dtype);
+  return v;
+}
 
 // h = act(g) u as operand planes (columns [hidden, ld) zero), g and u saved
 template <int ELEM, int NPH>
 struct GateEpi {
   static constexpr bool PAIR = true;
-  using State = NoState;
+  using State = Four;  // the bias of this lane's columns
   int act, hidden, hidden_p;  // hidden_p: hidden rounded up to 8
   int dtype;
   const void* bias;  // (2 hidden) or NULL
@@ -122,20 +133,21 @@ struct GateEpi {
   int64_t h_plane;
   float* gu;  // (rows, 2 hidden_p) or NULL
   template <class T>
-  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
+  __device__ __forceinline__ Four begin(int n0, int lane) const {
+    static_assert(64 % (T::WN / 8) == 0, "a lane keeps its columns");
+    const int n = n0 + lane % (T::WN / 8) * 4;
+    if (!bias || n >= hidden) return Four{};
+    return Four{load4(bias, n, hidden - n, dtype), load4(bias, (int64_t)hidden + n, hidden - n, dtype)};
+  }
+  template <class T>
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, const Four& b, int, int) const {
     each_piece<T, T::WN / 2>(buf, lane, [&](int r, int c, const f32x4* p) {
       const int m = m0 + r, n = n0 + c;
       if (m >= a.M || n >= hidden_p) return;
-      f32x4 g = *p, u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + T::WN / 2), h4;
+      const f32x4 g = *p + b.v, u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + T::WN / 2) + b.w;
+      f32x4 h4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = n + e < hidden;
-        if (bias && in) {
-          g[e] += load_as(bias, n + e, dtype);
-          u[e] += load_as(bias, (int64_t)hidden + n + e, dtype);
-        }
-        h4[e] = in ? act_only(act, g[e]) * u[e] : 0.f;
-      }
+      for (int e = 0; e < 4; ++e) h4[e] = n + e < hidden ? act_only(act, g[e]) * u[e] : 0.f;
       store_planes<ELEM, NPH>(h + (int64_t)m * hidden_p + n, h_plane, h4);
       if (gu) {
         float* o = gu + (int64_t)m * 2 * hidden_p + n;
@@ -145,7 +157,7 @@ struct GateEpi {
     });
   }
   template <class T>
-  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
+  __device__ __forceinline__ void finish(const Args&, int, int, const Four&, int, int) const {}
 };
 
 // acc = dh: dg = dh u act'(g), du = dh act(g) as operand planes side by side (rows of 2 hidden_p, padding zero), and, for the
@@ -162,6 +174,8 @@ struct GateBwdEpi {
   u16* d;  // (rows, 2 hidden_p)
   int64_t d_plane;
   float* partial;  // (tiles_m * WAVES_M, 2 hidden_p) or NULL
+  template <class T>
+  __device__ __forceinline__ ColumnSums begin(int, int) const { return ColumnSums{}; }
   template <class T>
   __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, ColumnSums& s, int, int) const {
     each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
@@ -211,38 +225,38 @@ struct GateBwdEpi {
 // [dg | du]^T x); the padding rows are not stored.
 struct OutEpi {
   static constexpr bool PAIR = false;
-  using State = NoState;
+  using State = Four;  // the bias of this lane's columns
   void* out;
   int64_t ld;
   int dtype;
   const void* bias;
   const void* res;
   int64_t ld_res;
-  int rows, gap_at, gap;
+  int rows, gap_at, gap, cols;
   int vec;  // rows of out are aligned for four elements at a time
-  __device__ __forceinline__ void put(int m, int n, int N, f32x4 v) const {
+  __device__ __forceinline__ f32x4 bias_at(int n) const { return bias && n < cols ? load4(bias, n, cols - n, dtype) : f32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void put(int m, int n, f32x4 v, f32x4 b) const {
     if (m >= gap_at) {
       if (m < gap_at + gap) return;
       m -= gap;
     }
-    if (m >= rows) return;
-    const int left = N - n;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < left) {
-        if (bias) v[e] += load_as(bias, n + e, dtype);
-        if (res) v[e] += load_as(res, (int64_t)m * ld_res + n + e, dtype);
-      }
+    if (m >= rows || n >= cols) return;
+    const int left = cols - n;
+    v += b;
+    if (res) v += load4(res, (int64_t)m * ld_res + n, left, dtype);
     store4(out, (int64_t)m * ld + n, dtype, v, left, vec);
   }
   template <class T>
-  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
-    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
-      if (m0 + r < a.M && n0 + c < a.N) put(m0 + r, n0 + c, a.N, *p);
-    });
+  __device__ __forceinline__ Four begin(int n0, int lane) const {
+    static_assert(64 % (T::WN / 4) == 0, "a lane keeps its columns");
+    return Four{bias_at(n0 + lane % (T::WN / 4) * 4), {}};
   }
   template <class T>
-  __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
+  __device__ __forceinline__ void emit(const Args&, float* buf, int m0, int n0, int lane, const Four& b, int, int) const {
+    each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) { put(m0 + r, n0 + c, *p, b.v); });
+  }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, const Four&, int, int) const {}
 };
 
 // fp32 partial sums of a product split along K: (splits, M, Np), Np = N rounded up to 4
@@ -251,6 +265,8 @@ struct PartialEpi {
   using State = NoState;
   float* partial;
   int Np;
+  template <class T>
+  __device__ __forceinline__ NoState begin(int, int) const { return {}; }
   template <class T>
   __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
     float* base = partial + (int64_t)blockIdx.z * a.M * Np;
@@ -264,13 +280,14 @@ struct PartialEpi {
 };
 
 // joins the splits in order and finishes the output
-static __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, int M, int N, int Np,
+static __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, int M, int Np,
                                                    const OutEpi epi) {
   const int64_t per = Np / 4, total = (int64_t)M * per;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
     f32x4 s = {0, 0, 0, 0};
     for (int z = 0; z < splits; ++z) s += *reinterpret_cast<const f32x4*>(partial + (int64_t)z * M * Np + t * 4);
-    epi.put((int)(t / per), (int)(t % per) * 4, N, s);
+    const int n = (int)(t % per) * 4;
+    epi.put((int)(t / per), n, s, epi.bias_at(n));
   }
 }
 
@@ -451,7 +468,7 @@ void product_out(const Args& a, const OutEpi& epi, float* partial, hipStream_t s
   const int used = (k_tiles + per - 1) / per;  // (every share has work)
   launch<Small>(a, PartialEpi{partial, Np}, a.N, used, s);
   const int64_t threads = (int64_t)a.M * (Np / 4), blocks = (threads + 255) / 256;
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, partial, used, a.M, a.N, Np, epi);
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, partial, used, a.M, Np, epi);
 }
 
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
@@ -493,7 +510,7 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   const Operand hop{h, p.Fp, h_plane, 0};
   product_out<ELEM, NPH, NPL, true, true>(
       args_of(hop, w_out, p.M, p.O, p.Fp),
-      OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, vec_ok(d->y, d->ld_y, p.dtype)}, partial, s);
+      OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, p.O, vec_ok(d->y, d->ld_y, p.dtype)}, partial, s);
   return ws.off;
 }
 
@@ -545,12 +562,12 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   }
   const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
   const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};
-  auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g) {
-    return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, vec_ok(q, ld, p.dtype)};
+  auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g, int cols) {
+    return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, cols, vec_ok(q, ld, p.dtype)};
   };
-  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0), partial, s);
-  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap), partial, s);
-  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0), partial, s);
+  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0, p.K), partial, s);
+  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), partial, s);
+  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), partial, s);
   return ws.off;
 }
 

@@ -113,6 +113,8 @@ struct Tile {
   static constexpr int LOADS = (NPA * CA + NPB * CB) / NT;    // per thread and stage
   static constexpr int ROW = WN + 4;                          // floats of an epilogue row in LDS (the padding spreads the banks)
   static constexpr int ROWS_BYTES = 32 * ROW * 4, ROWS_PER_STAGE = STAGE * 16 / ROWS_BYTES;
+  static constexpr bool TURNS = NW == 8 && STAGES == 2;                // two waves per SIMD, taking turns (product_kernel)
+  static constexpr int TURN_K = NPA == 1 && NPB == 1 ? 2 : 1;          // MFMA steps of a turn
   static_assert(BK == 32 || BK == 64, "K step");
   static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * LOADS < 64, "loads in flight");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS");
@@ -292,7 +294,8 @@ __device__ __forceinline__ void each_turned_piece(const float* buf, int lane, co
 // The second operand's rows are the MFMA's first operand: four accumulator elements of a lane are four consecutive columns of
 // one row.  The epilogue gets the tile 32 rows of a wave at a time, turned through LDS so that consecutive lanes hold
 // consecutive pieces of a row: its loads and stores then cover whole cache lines.
-// Epi: emit(a, buf, m0, n0, lane, state, tm, tn) for every 32 rows, finish(...) once; Epi::PAIR: columns [0, WN / 2) of buf are the
+// Epi: begin(n0, lane) once -> state (a lane's column does not change), emit(a, buf, m0, n0, lane, state, tm, tn) for every 32 rows,
+// finish(...) once; Epi::PAIR: columns [0, WN / 2) of buf are the
 // first half's, [WN / 2, WN) the second's.
 template <class T, class Epi>
 __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const Epi epi) {
@@ -374,39 +377,74 @@ __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const E
           }
       }
   };
-  auto step = [&](u32x4* cur, const u32x4* nxt, int kt) {
+  if constexpr (T::TURNS) {
+    // Two waves per SIMD take turns (8192 x 10240 x 4096 in bf16: 532 -> 516 us, 4096^3 in three planes 573 -> 558): while one multiplies, the other fetches its next fragments.  Waves 4..7 run one turn (a
+    // barrier) behind waves 0..3.  Turn pair t of a K tile: fetch KT MFMA steps of fragments | barrier | multiply them | barrier.
+    // The stage read last is refilled in the first turn of the next tile (both halves have left it by then); a wave's own loads
+    // of the next stage have landed before the barrier behind its last fetch of this one, one turn before anybody reads it.
+    constexpr int KT = T::TURN_K, NT = T::BK / 16 / KT;
+    const bool second = wave >= T::NW / 2;
+    issue(st0, kt0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    barrier();
+    if (second) barrier();
+    auto step = [&](const u32x4* cur, u32x4* nxt, int kt) {
 #pragma unroll
-    for (int kk = 0; kk < T::BK / 16; ++kk) {
-      if (kk + 1 < T::BK / 16) {
-        fetch(cur, kk + 1, (kk + 1) & 1);
-      } else {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
+      for (int t = 0; t < NT; ++t) {
+        if (t == 0) issue(nxt, kt + 1);
+#pragma unroll
+        for (int k = 0; k < KT; ++k) fetch(cur, t * KT + k, k);
+        if (t == NT - 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         barrier();
-        issue(cur, kt + S);
-        fetch(nxt, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < KT; ++k) multiply(k);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        barrier();
       }
-      multiply(kk & 1);
-    }
-  };
-
-  issue(st0, kt0);
-  issue(st1, kt0 + 1);
-  if constexpr (S > 2) issue(st2, kt0 + 2);
-  if constexpr (S > 3) issue(st3, kt0 + 3);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * T::LOADS) : "memory");
-  barrier();
-  fetch(st0, 0, 0);
-  for (int kt = kt0; kt < kt1; kt += S) {
-    step(st0, st1, kt);
-    if constexpr (S == 2) {
+    };
+    for (int kt = kt0; kt < kt1; kt += 2) {
+      step(st0, st1, kt);
       if (kt + 1 < kt1) step(st1, st0, kt + 1);
-    } else {
-      if (kt + 1 < kt1) step(st1, st2, kt + 1);
-      if constexpr (S == 3) {
-        if (kt + 2 < kt1) step(st2, st0, kt + 2);
+    }
+    if (!second) barrier();
+  } else {
+    auto step = [&](u32x4* cur, const u32x4* nxt, int kt) {
+#pragma unroll
+      for (int kk = 0; kk < T::BK / 16; ++kk) {
+        if (kk + 1 < T::BK / 16) {
+          fetch(cur, kk + 1, (kk + 1) & 1);
+        } else {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
+          barrier();
+          issue(cur, kt + S);
+          fetch(nxt, 0, 0);
+        }
+        multiply(kk & 1);
+      }
+    };
+
+    issue(st0, kt0);
+    issue(st1, kt0 + 1);
+    if constexpr (S > 2) issue(st2, kt0 + 2);
+    if constexpr (S > 3) issue(st3, kt0 + 3);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * T::LOADS) : "memory");
+    barrier();
+    fetch(st0, 0, 0);
+    for (int kt = kt0; kt < kt1; kt += S) {
+      step(st0, st1, kt);
+      if constexpr (S == 2) {
+        if (kt + 1 < kt1) step(st1, st0, kt + 1);
       } else {
-        if (kt + 2 < kt1) step(st2, st3, kt + 2);
-        if (kt + 3 < kt1) step(st3, st0, kt + 3);
+        if (kt + 1 < kt1) step(st1, st2, kt + 1);
+        if constexpr (S == 3) {
+          if (kt + 2 < kt1) step(st2, st0, kt + 2);
+        } else {
+          if (kt + 2 < kt1) step(st2, st3, kt + 2);
+          if (kt + 3 < kt1) step(st3, st0, kt + 3);
+        }
       }
     }
   }
@@ -421,11 +459,13 @@ __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const E
 
   // this wave's 32 epilogue rows lie in one of the stages, which nobody reads any more
   const int slot = wave / T::ROWS_PER_STAGE, in = wave % T::ROWS_PER_STAGE;
-  u32x4* st = slot == 0 ? st0 : slot == 1 ? st1 : slot == 2 ? st2 : st3;
+  u32x4* st = slot == 0 ? st0 : st1;
+  if constexpr (S > 2) st = slot == 2 ? st2 : st;
+  if constexpr (S > 3) st = slot == 3 ? st3 : st;
   float* buf = reinterpret_cast<float*>(st) + in * 32 * T::ROW;
   const int li = lane & 31, lh = lane >> 5;
   const int m0 = row0 + wm * T::WM, n0 = col0 + wn * (Epi::PAIR ? T::WN / 2 : T::WN);
-  typename Epi::State state{};
+  typename Epi::State state = epi.template begin<T>(n0, lane);
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
 #pragma unroll

@@ -120,6 +120,8 @@ template <int NPL>
 struct SymEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
   using State = NoState;
+  template <class T>
+  __device__ __forceinline__ NoState begin(int, int) const { return {}; }
   float alpha, beta;
   const u16* add;  // or NULL
   u16* out;
@@ -152,6 +154,8 @@ struct SymEpi {
 struct SymPartialEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
   using State = NoState;
+  template <class T>
+  __device__ __forceinline__ NoState begin(int, int) const { return {}; }
   float* partial;
   int size, ld;
   template <class T>
@@ -192,6 +196,8 @@ __global__ __launch_bounds__(256) void sym_join_kernel(const float* __restrict__
 struct StepEpi {
   [[maybe_unused]] static constexpr bool PAIR = false;
   using State = NoState;
+  template <class T>
+  __device__ __forceinline__ NoState begin(int, int) const { return {}; }
   float a, alpha;
   const u16* x;
   u16* out;
