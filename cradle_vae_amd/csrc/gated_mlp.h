@@ -21,28 +21,37 @@ using namespace mm16;
 
 enum Act { SILU = 0, GELU = 1 };
 
-// act(g) and act'(g).  silu: g s, s = 1 / (1 + exp(-g)); gelu: g Phi(g), Phi through erf.
+// act(g) and act'(g), in a handful of instructions: an epilogue has one or two waves per SIMD and nothing to hide long sequences
+// behind (with the library's expf, erfcf and divisions the first backward product of 1537 x 1000 x 2731 takes 45 us).
+// silu: g s, s = 1 / (1 + exp(-g)) on the hardware's exp2 and reciprocal, a few 2^-24 relative.
+// gelu: g Phi(g), Phi(-|g|) = (a1 t + ... + a5 t^5) exp(-g^2 / 2) / 2, t = 1 / (1 + 0.3275911 |g| / sqrt(2)): the rational
+// approximation 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions, off by at most 0.75e-7.
+// Limits: a gate of 0 with its argument infinite is 0.
+__device__ __forceinline__ float sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
+}
+// Phi(g); e = exp(-g^2 / 2)
+__device__ __forceinline__ float normal_cdf(float g, float e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.23164188f, fabsf(g), 1.f));
+  const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f) * e;
+  return g < 0.f ? q : 1.f - q;
+}
 __device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
   if (act == SILU) {
-    const float s = 1.f / (1.f + expf(-g));
-    // (g s with s = 0 and g = -inf is 0 * inf: the limit is 0)
+    const float s = sigmoid(g);
     a = s == 0.f ? 0.f : g * s;
-    da = s == 0.f ? 0.f : s * (1.f + g * (1.f - s));
+    da = s == 0.f ? 0.f : s * fmaf(g, 1.f - s, 1.f);
     if (g == INFINITY) da = 1.f;
   } else {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-    const float pdf = 0.39894228040143268f * expf(-0.5f * g * g);
+    const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
+    const float cdf = normal_cdf(g, e);
     a = cdf == 0.f ? 0.f : g * cdf;
-    da = pdf == 0.f ? cdf : cdf + g * pdf;
+    da = e == 0.f ? cdf : fmaf(g * 0.39894228040143268f, e, cdf);
   }
 }
 __device__ __forceinline__ float act_only(int act, float g) {
-  if (act == SILU) {
-    const float s = 1.f / (1.f + expf(-g));
-    return s == 0.f ? 0.f : g * s;
-  }
-  const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-  return cdf == 0.f ? 0.f : g * cdf;
+  const float s = act == SILU ? sigmoid(g) : normal_cdf(g, __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g));
+  return s == 0.f ? 0.f : g * s;
 }
 
 // ---------------------------------------------------------------------------------------------------------------

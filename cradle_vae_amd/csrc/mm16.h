@@ -276,6 +276,21 @@ __device__ __forceinline__ void each_piece(float* buf, int lane, const Fn& fn) {
   }
 }
 
+// The same with what memory holds for each piece: all of load(row, column) first, so that the loads are in flight together (a
+// store between them would make each wait for the one before), then fn(row, column, piece, loaded).
+template <class T, int W, class Load, class Fn>
+__device__ __forceinline__ void each_piece(float* buf, int lane, const Load& load, const Fn& fn) {
+  constexpr int P = W / 4, IT = 32 * P / 64;
+  decltype(load(0, 0)) v[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) v[it] = load((it * 64 + lane) / P, (it * 64 + lane) % P * 4);
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int r = (it * 64 + lane) / P, c = (it * 64 + lane) % P * 4;
+    fn(r, c, reinterpret_cast<f32x4*>(buf + r * T::ROW + c), v[it]);
+  }
+}
+
 // The same, turned: four rows of one column, consecutive lanes consecutive rows: fn(first row, column, numbers)
 template <class T, int W, class Fn>
 __device__ __forceinline__ void each_turned_piece(const float* buf, int lane, const Fn& fn) {

@@ -102,17 +102,23 @@ __global__ __launch_bounds__(256) void pack_kernel(const Tensor g, const double*
   }
 }
 
-// four consecutive numbers of a two-plane matrix (or of its hi plane)
-template <int NPL = 2>
-__device__ __forceinline__ f32x4 load_planes(const u16* p, int64_t plane) {
-  const u32x2 h = *reinterpret_cast<const u32x2*>(p);
-  if constexpr (NPL == 1) return f32x4{from_f16((u16)h.x), from_f16((u16)(h.x >> 16)), from_f16((u16)h.y), from_f16((u16)(h.y >> 16))};
-  const u32x2 l = *reinterpret_cast<const u32x2*>(p + plane);
-  return f32x4{from_f16((u16)h.x) + from_f16((u16)l.x), from_f16((u16)(h.x >> 16)) + from_f16((u16)(l.x >> 16)),
-               from_f16((u16)h.y) + from_f16((u16)l.y), from_f16((u16)(h.y >> 16)) + from_f16((u16)(l.y >> 16))};
+struct NoState {};
+// four consecutive numbers of a two-plane matrix (NPL = 1: of its hi plane)
+struct Raw {
+  u32x2 h, l;
+};
+template <int NPL>
+__device__ __forceinline__ Raw load_raw(const u16* p, int64_t plane) {
+  return Raw{*reinterpret_cast<const u32x2*>(p), NPL == 2 ? *reinterpret_cast<const u32x2*>(p + plane) : u32x2{0, 0}};
+}
+template <int NPL>
+__device__ __forceinline__ f32x4 value_of(const Raw& r) {
+  f32x4 v = {from_f16((u16)r.h.x), from_f16((u16)(r.h.x >> 16)), from_f16((u16)r.h.y), from_f16((u16)(r.h.y >> 16))};
+  if constexpr (NPL == 2) v += f32x4{from_f16((u16)r.l.x), from_f16((u16)(r.l.x >> 16)), from_f16((u16)r.l.y), from_f16((u16)(r.l.y >> 16))};
+  return v;
 }
 
-struct NoState {};
+__device__ __forceinline__ f32x4 load_planes(const u16* p, int64_t plane) { return value_of<2>(load_raw<2>(p, plane)); }
 
 // out = alpha acc + beta add, a symmetric matrix of `size` rows, ld = size rounded up to 8 (padding columns zero).  Tiles below the
 // diagonal are stored a second time, turned, above it.
@@ -127,9 +133,14 @@ struct SymEpi {
   u16* out;
   int64_t plane, batch;
   int size, ld;
-  __device__ __forceinline__ f32x4 value(int m, int n, f32x4 v) const {
+  // what is added at (m, n) (places beyond the matrix: its last, not used)
+  __device__ __forceinline__ Raw addend(int m, int n) const {
+    if (!add) return Raw{};
+    return load_raw<NPL>(add + (int64_t)blockIdx.y * batch + (int64_t)min(m, size - 1) * ld + min(n, ld - 4), plane);
+  }
+  __device__ __forceinline__ f32x4 value(int m, int n, f32x4 v, const Raw& r) const {
     v *= alpha;
-    if (m < size && n < ld && add) v += beta * load_planes<NPL>(add + (int64_t)blockIdx.y * batch + (int64_t)m * ld + n, plane);
+    if (m < size && n < ld && add) v += beta * value_of<NPL>(r);
     return v;
   }
   __device__ __forceinline__ void put(int row, int col, f32x4 v) const {
@@ -137,8 +148,9 @@ struct SymEpi {
   }
   template <class T>
   __device__ __forceinline__ void emit(const Args&, float* buf, int m0, int n0, int lane, NoState&, int tm, int tn) const {
-    each_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4* p) {
-      const f32x4 v = value(m0 + r, n0 + c, *p);
+    const auto load = [&](int r, int c) { return addend(m0 + r, n0 + c); };
+    each_piece<T, T::WN>(buf, lane, load, [&](int r, int c, f32x4* p, const Raw& old) {
+      const f32x4 v = value(m0 + r, n0 + c, *p, old);
       put(m0 + r, n0 + c, v);
       *p = v;
     });
@@ -183,7 +195,7 @@ __global__ __launch_bounds__(256) void sym_join_kernel(const float* __restrict__
 #pragma unroll 4
     for (int z = 0; z < splits; ++z) v += *reinterpret_cast<const f32x4*>(p + z * per);
   }
-  v = epi.value(m, n, v);
+  v = epi.value(m, n, v, epi.addend(m, n));
   epi.put(m, n, v);
   if (n0 / tile == m0 / tile) return;
 #pragma unroll
@@ -209,10 +221,11 @@ struct StepEpi {
   template <class T>
   __device__ __forceinline__ void emit(const Args& ar, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
     const int64_t b = (int64_t)blockIdx.y * batch, br = (int64_t)blockIdx.y * batch_result;
-    each_piece<T, T::WN>(buf, lane, [&](int r, int c, f32x4* p) {
+    const auto load = [&](int r, int c) { return load_raw<2>(x + b + (int64_t)min(m0 + r, ar.M - 1) * ld + min(n0 + c, ld - 4), plane); };
+    each_piece<T, T::WN>(buf, lane, load, [&](int r, int c, f32x4* p, const Raw& old) {
       const int m = m0 + r, n = n0 + c;
       if (m >= ar.M || n >= ld) return;
-      const f32x4 v = alpha * *p + a * load_planes(x + b + (int64_t)m * ld + n, plane);
+      const f32x4 v = alpha * *p + a * value_of<2>(old);
       if (!result) store_planes<F16, 2>(out + b + (int64_t)m * ld + n, plane, v);
       else if (flip) *p = v * (1.f / kScale);
       else store4(result, br + (int64_t)m * ld_result + n, dtype, v * (1.f / kScale), ar.N - n, vec);
