@@ -288,18 +288,6 @@ struct PartialEpi {
   __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
-// joins the splits in order and finishes the output
-static __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, int M, int Np,
-                                                   const OutEpi epi) {
-  const int64_t per = Np / 4, total = (int64_t)M * per;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    f32x4 s = {0, 0, 0, 0};
-    for (int z = 0; z < splits; ++z) s += *reinterpret_cast<const f32x4*>(partial + (int64_t)z * M * Np + t * 4);
-    const int n = (int)(t % per) * 4;
-    epi.put((int)(t / per), n, s, epi.bias_at(n));
-  }
-}
-
 // column sums in two passes with a fixed order.  First: blockIdx.y-th share of the rows of a (rows, cols) tensor, eight rows'
 // loads in flight per thread.
 template <int DT>
@@ -322,23 +310,65 @@ static __global__ __launch_bounds__(256) void colsum_kernel(const void* __restri
   if (w == 0 && c < cols)
     partial[(int64_t)blockIdx.y * cols + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
-// Second: sums `n` partial rows of `ld` floats; columns [0, cols), of which those from gap_at on are read gap further right
-static __global__ __launch_bounds__(1024) void colsum_join_kernel(const float* __restrict__ partial, int n, int ld, int cols,
-                                                                  int gap_at, int gap, void* __restrict__ out, int dtype) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  __shared__ float red[16][64];
-  float s = 0.f;
-  if (c < cols) {
-    const float* p = partial + c + (c >= gap_at ? gap : 0);
+
+// What is left to do once the products of a pass are done, in one launch: joining products split along K (partial sums in the
+// order of the splits, then the output's epilogue) and the second passes of column sums (partial rows in a fixed order; columns from
+// gap_at on are read gap further right).
+struct FinishJob {
+  const float* partial;
+  int n, ld;         // splits / partial rows; floats of a row
+  int M;             // rows of the output (0: a column sum)
+  int cols, gap_at, gap;
+  OutEpi out;        // its tensor is the column sums' output too
+  int first, blocks; // workgroups
+};
+struct Finish {
+  FinishJob job[5];
+  int n = 0, blocks = 0;
+  void add(const FinishJob& j, int64_t blocks_of_job) {
+    job[n] = j;
+    job[n].first = blocks;
+    job[n].blocks = (int)blocks_of_job;
+    blocks += job[n].blocks;
+    ++n;
+  }
+};
+static __global__ __launch_bounds__(256) void finish_kernel(const Finish f) {
+  int k = 0;
+  while (k + 1 < f.n && (int)blockIdx.x >= f.job[k + 1].first) ++k;
+  const FinishJob& j = f.job[k];
+  const int block = blockIdx.x - j.first;
+  if (j.M) {
+    const int64_t per = j.ld / 4, total = (int64_t)j.M * per, stride = (int64_t)j.M * j.ld;
+    for (int64_t t = (int64_t)block * 256 + threadIdx.x; t < total; t += (int64_t)j.blocks * 256) {
+      f32x4 s = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int r = w; r < n; r += 16) s += p[(int64_t)r * ld];
+      for (int z = 0; z < j.n; ++z) s += *reinterpret_cast<const f32x4*>(j.partial + z * stride + t * 4);
+      const int n = (int)(t % per) * 4;
+      j.out.put((int)(t / per), n, s, j.out.bias_at(n));
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = block * 64 + lane;
+  __shared__ float red[4][64];
+  float s = 0.f;
+  if (c < j.cols) {
+    const float* p = j.partial + c + (c >= j.gap_at ? j.gap : 0);
+#pragma unroll 8
+    for (int r = w; r < j.n; r += 4) s += p[(int64_t)r * j.ld];
   }
   red[w][lane] = s;
   __syncthreads();
-  if (w != 0 || c >= cols) return;
-#pragma unroll
-  for (int k = 1; k < 16; ++k) s += red[k][lane];
-  store_as(out, c, dtype, s);
+  if (w == 0 && c < j.cols) store_as(j.out.out, c, j.out.dtype, (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+}
+inline void run_finish(const Finish& f, hipStream_t s) {
+  if (f.n) hipLaunchKernelGGL(finish_kernel, dim3(f.blocks), dim3(256), 0, s, f);
+}
+inline void add_column_sums(Finish& f, const float* partial, int n, int ld, int cols, int gap_at, int gap, void* out, int dtype) {
+  FinishJob j{};
+  j.partial = partial, j.n = n, j.ld = ld, j.cols = cols, j.gap_at = gap_at, j.gap = gap;
+  j.out.out = out, j.out.dtype = dtype;
+  f.add(j, (cols + 63) / 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -467,8 +497,9 @@ int splits_of(const Args& a) {
   return (int)(want < most ? want : most);
 }
 
+// the product into its tensor, or into partial sums that `finish` joins
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
-void product_out(const Args& a, const OutEpi& epi, float* partial, hipStream_t s) {
+void product_out(const Args& a, const OutEpi& epi, float* partial, Finish& finish, hipStream_t s) {
   const int splits = splits_of<ELEM, NPA, NPB, AK, BK>(a);
   if (splits == 1) return product<ELEM, NPA, NPB, AK, BK>(a, epi, a.N, s);
   using Small = typename Tiles<ELEM, NPA, NPB, AK, BK>::Small;
@@ -476,8 +507,10 @@ void product_out(const Args& a, const OutEpi& epi, float* partial, hipStream_t s
   const int k_tiles = (a.K + Small::BK - 1) / Small::BK, per = (k_tiles + splits - 1) / splits;
   const int used = (k_tiles + per - 1) / per;  // (every share has work)
   launch<Small>(a, PartialEpi{partial, Np}, a.N, used, s);
-  const int64_t threads = (int64_t)a.M * (Np / 4), blocks = (threads + 255) / 256;
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, partial, used, a.M, Np, epi);
+  FinishJob j{};
+  j.partial = partial, j.n = used, j.ld = Np, j.M = a.M, j.out = epi;
+  const int64_t blocks = ((int64_t)a.M * (Np / 4) + 255) / 256;
+  finish.add(j, blocks < 1024 ? blocks : 1024);
 }
 
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
@@ -517,9 +550,11 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   product<ELEM, NPL, NPL, true, true>(
       a, GateEpi<ELEM, NPH>{d->act, p.F, p.Fp, p.dtype, d->b_in, h, h_plane, static_cast<float*>(d->saved_gu)}, p.F, s);
   const Operand hop{h, p.Fp, h_plane, 0};
+  Finish finish;
   product_out<ELEM, NPH, NPL, true, true>(
       args_of(hop, w_out, p.M, p.O, p.Fp),
-      OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, p.O, vec_ok(d->y, d->ld_y, p.dtype)}, partial, s);
+      OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, p.O, vec_ok(d->y, d->ld_y, p.dtype)}, partial, finish, s);
+  run_finish(finish, s);
   return ws.off;
 }
 
@@ -529,7 +564,7 @@ inline int colsum_rows(int rows) {
   return most > kColsumRows ? most : kColsumRows;
 }
 
-// ---- backward: workspace = packed x, W_in, W_out, dy | [dg | du] | partial sums | column-sum partials
+// ---- backward: workspace = packed x, W_in, W_out, dy | [dg | du] | partial sums of dx, dW_in, dW_out | of the column sums
 template <int ELEM, int NPL, int NPH>
 int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, hipStream_t s, bool run) {
   Bump ws{static_cast<char*>(workspace)};
@@ -542,12 +577,9 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp, d_plane = 2 * h_plane;
   u16* dgu = static_cast<u16*>(ws.take(d_plane * NPH * 2));
-  int64_t pf = partial_floats<ELEM, NPH, NPL, true, false>(p.M, p.K, 2 * p.Fp);
-  const int64_t pf1 = partial_floats<ELEM, NPH, NPL, false, false>(2 * p.Fp, p.K, p.M);
-  const int64_t pf2 = partial_floats<ELEM, NPL, NPH, false, false>(p.O, p.F, p.M);
-  pf = pf > pf1 ? pf : pf1;
-  pf = pf > pf2 ? pf : pf2;
-  float* partial = static_cast<float*>(ws.take(pf * 4));
+  float* p_dx = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, false>(p.M, p.K, 2 * p.Fp) * 4));
+  float* p_in = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, false, false>(2 * p.Fp, p.K, p.M) * 4));
+  float* p_out = static_cast<float*>(ws.take(partial_floats<ELEM, NPL, NPH, false, false>(p.O, p.F, p.M) * 4));
   const int sum_rows = (p.M + 127) / 128 * 4;  // of either tile size: 128 rows are at most four wave rows
   float* sums = static_cast<float*>(ws.take(d->db_in ? (int64_t)sum_rows * 2 * p.Fp * 4 : 0));
   const int per = colsum_rows(p.M), shares = (p.M + per - 1) / per;
@@ -560,23 +592,25 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   const bool large = use_large<typename TT::Large, typename TT::Small>(a, p.F, false);
   product<ELEM, NPL, NPL, true, false>(
       a, GateBwdEpi<ELEM, NPH>{d->act, p.F, p.Fp, static_cast<const float*>(d->saved_gu), dgu, d_plane, d->db_in ? sums : nullptr}, p.F, s);
+  Finish finish;
   if (d->db_in) {
     const int used = large ? (p.M + 255) / 256 * TT::Large::WAVES_M : (p.M + 127) / 128 * TT::Small::WAVES_M;
-    hipLaunchKernelGGL(colsum_join_kernel, dim3((2 * p.F + 63) / 64), dim3(1024), 0, s, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
+    add_column_sums(finish, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
   }
   if (d->db_out) {
     constexpr int DT = NPL == 3 ? CRADLE_F32 : ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
     hipLaunchKernelGGL(colsum_kernel<DT>, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.M, p.O, per, sums_out);
-    hipLaunchKernelGGL(colsum_join_kernel, dim3((p.O + 63) / 64), dim3(1024), 0, s, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
+    add_column_sums(finish, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
   }
   const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
   const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};
   auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g, int cols) {
     return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, cols, vec_ok(q, ld, p.dtype)};
   };
-  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0, p.K), partial, s);
-  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), partial, s);
-  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), partial, s);
+  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0, p.K), p_dx, finish, s);
+  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), p_in, finish, s);
+  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), p_out, finish, s);
+  run_finish(finish, s);
   return ws.off;
 }
 
