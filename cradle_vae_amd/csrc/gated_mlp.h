@@ -63,7 +63,7 @@ struct PackJob {
   int64_t ld_src, plane;
   int rows, cols, rows_dst, ld_dst;
   int gap_at, gap;  // destination rows [gap_at, gap_at + gap) are zero, and so are those behind the source's last
-  int vec;          // fp32 source with 16-byte aligned rows
+  int vec;          // the source's rows start on 16 bytes
 };
 struct PackJobs {
   PackJob job[4];
@@ -99,8 +99,14 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackJobs js) {
     } else {  // the numbers as they are
       const u16* q = static_cast<const u16*>(j.src) + s;
       u16 v[8];
+      if (j.vec && c0 + 8 <= j.cols) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(q + c0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = q[min(c0 + e, j.cols - 1)];
+        for (int e = 0; e < 8; ++e) v[e] = (u16)(a[e / 2] >> 16 * (e % 2));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = q[min(c0 + e, j.cols - 1)];
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e][0] = !zero && c0 + e < j.cols ? v[e] : (u16)0;
     }
@@ -386,10 +392,19 @@ constexpr int kCUs = 256;
 constexpr int64_t kSmallWork = 1LL << 28;
 
 struct Plan {
-  int M, K, F, O, Fp;
+  int M, K, F, O;
+  int Fp;                // row length of h and of each half of [dg | du]
   int dtype, elem, npl;  // planes of the tensors' operands
   int nph;               // planes of h and [dg | du]: twice a 16-bit tensor's bits while that is free
 };
+
+// A K tile's share of a row, in elements: rows that start on a multiple of it are staged in whole cache lines (three planes: half
+// lines).  1537 x 5462 x 1000 on one plane: 40.5 us with rows of 1000, 32.5 us with rows of 1024; 2560 x 1600 x 400 on three: 28.6
+// and 25.8 us.
+inline int line_of(int planes) { return planes == 3 ? 32 : 64; }
+// Rows that a 16-bit operand with other rows meets in a product along its own ones, from which on it is packed into such rows: a
+// fifth of 2 rows cols other / 600 TFLOP/s is then more than the packing's 4 rows cols bytes at 5 TB/s.
+constexpr int kManyRows = 2048;
 
 inline Plan plan_of(const cradle_gated_mlp_desc* d) {
   Plan p;
@@ -397,10 +412,13 @@ inline Plan plan_of(const cradle_gated_mlp_desc* d) {
   p.K = d->width;
   p.F = d->hidden;
   p.O = d->out_width;
-  p.Fp = (int)up8(p.F);
   p.dtype = d->dtype;
   p.elem = d->dtype == CRADLE_F16 ? F16 : BF16;
   p.npl = d->dtype == CRADLE_F32 ? 3 : 1;
+  const int run = line_of(p.npl);
+  // (the padding is multiplied too: at most a 16th; a 16-bit W_in that a gap would have to be packed for stays as it is for few rows)
+  const bool packs = p.npl == 3 || p.F % 8 != 0 || p.M >= kManyRows;
+  p.Fp = packs && p.F >= 16 * run ? (p.F + run - 1) / run * run : (int)up8(p.F);
   p.nph = p.npl == 1 && (int64_t)p.M * p.F * (p.K + p.O) < kSmallWork ? 2 : p.npl;
   return p;
 }
@@ -421,13 +439,15 @@ struct Bump {
 };
 
 // operand of tensor `src` (rows x cols): itself, or packed into the workspace (a job is queued)
-// with rows_dst rows, gap of them between the two halves
-inline Operand operand(const Plan& p, const void* src, int64_t ld, int rows, int cols, int rows_dst, int gap_at, int gap, Bump& ws,
-                PackJobs& js, int& n_jobs) {
-  if (direct(src, ld, cols, p.dtype) && gap == 0) return {static_cast<const u16*>(src), ld, 0, 0};
-  const int64_t ldp = up8(cols), plane = (int64_t)rows_dst * ldp;
+// with rows_dst rows, gap of them between the two halves.  other: rows it meets in a product along its own rows (0: none such).
+inline Operand operand(const Plan& p, const void* src, int64_t ld, int rows, int cols, int rows_dst, int gap_at, int gap, int other, Bump& ws,
+                       PackJobs& js, int& n_jobs) {
+  const int run = line_of(p.npl);
+  if (direct(src, ld, cols, p.dtype) && gap == 0 && (ld % run == 0 || other < kManyRows)) return {static_cast<const u16*>(src), ld, 0, 0};
+  const int64_t ldp = (cols + run - 1) / run * run, plane = (int64_t)rows_dst * ldp;
   u16* dst = static_cast<u16*>(ws.take(plane * p.npl * 2));
-  js.job[n_jobs++] = {src, dst, ld, plane, rows, cols, rows_dst, (int)ldp, gap_at, gap, ld % 4 == 0 && ((uintptr_t)src & 15) == 0};
+  js.job[n_jobs++] = {src, dst, ld, plane, rows, cols, rows_dst, (int)ldp, gap_at, gap,
+                      ld % (p.npl == 3 ? 4 : 8) == 0 && ((uintptr_t)src & 15) == 0};
   return {dst, ldp, plane, 0};
 }
 
@@ -537,9 +557,9 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   PackJobs js{};
   int n = 0;
   const int gap = p.Fp - p.F;
-  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, ws, js, n);
-  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, ws, js, n);
-  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
+  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, 2 * p.F, ws, js, n);
+  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, p.M, ws, js, n);
+  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, p.M, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp;
   u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * NPH * 2));
   float* partial = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, true>(p.M, p.O, p.Fp) * 4));
@@ -571,10 +591,10 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   PackJobs js{};
   int n = 0;
   const int gap = p.Fp - p.F;
-  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, ws, js, n);
-  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, ws, js, n);
-  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, ws, js, n);
-  const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, ws, js, n);
+  const Operand x = operand(p, d->x, d->ld_x, p.M, p.K, p.M, kNoGap, 0, 0, ws, js, n);
+  const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, 0, ws, js, n);
+  const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, 0, ws, js, n);
+  const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, p.F, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp, d_plane = 2 * h_plane;
   u16* dgu = static_cast<u16*>(ws.take(d_plane * NPH * 2));
   float* p_dx = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, false>(p.M, p.K, 2 * p.Fp) * 4));
