@@ -384,7 +384,7 @@ inline int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 inline int esize(int dtype) { return dtype == CRADLE_F32 ? 4 : 2; }
 
-constexpr int kFewRows = 4;   // rows up to which the weights' reading bounds the block (measured beside few_rows)
+constexpr int kFewRows = 8;   // (few_rows)
 constexpr int kCUs = 256;
 
 // Below this many products per projection (2^28: under 2 us of the matrix cores) a block's time is its launches, and the second

@@ -122,7 +122,14 @@ int64_t backward_of(const cradle_gated_mlp_desc* d, const Plan& p, hipStream_t s
   return (p.dtype == CRADLE_F16 ? backward_f16 : p.dtype == CRADLE_BF16 ? backward_bf16 : backward_f32)(d, p, run ? d->workspace : nullptr, s, run);
 }
 
-bool few_rows(const cradle_gated_mlp_desc* d) { return d->rows <= kFewRows && !d->saved_gu; }
+// The rows for which dot products beat the tile products, whose time hardly depends on so few rows.  Dot products | tiles in us,
+// width x hidden: 4096 x 10240 in bf16, 1 row 41 | 70, 4 rows 66 | 63, 8 rows 96 | 72 (one row reads 252 MB of weights at 6.2 TB/s,
+// partly from the last-level cache; each further one adds 8 us of arithmetic); 1024 x 2560 in bf16, 1 row 6 | 19, 8 rows 20 | 20;
+// 512 x 1024 in fp32, 1 row 5 | 28, 8 rows 15 | 28.
+bool few_rows(const cradle_gated_mlp_desc* d) {
+  const int64_t weights = (int64_t)d->hidden * (2 * d->width + (int64_t)d->out_width);
+  return !d->saved_gu && d->rows <= (weights < (1 << 24) ? kFewRows : kFewRows / 2);
+}
 
 int check_desc(const cradle_gated_mlp_desc* d, const char* what) {
   CRADLE_CHECK_ARG(d, "%s: null descriptor", what);
@@ -133,7 +140,8 @@ int check_desc(const cradle_gated_mlp_desc* d, const char* what) {
   // 32-bit byte offsets inside a tile (mm16.h) and int element counts of the tile grids
   CRADLE_CHECK_ARG(d->width <= (1 << 20) && d->hidden <= (1 << 20) && d->out_width <= (1 << 20) && d->rows <= (1 << 24),
                    "%s: rows <= 2^24, widths <= 2^20 (got %d, %d, %d, %d)", what, d->rows, d->width, d->hidden, d->out_width);
-  CRADLE_CHECK_ARG(((int64_t)d->hidden + 264) * (d->ld_w_in > d->width ? up8(d->ld_w_in) : up8(d->width)) < (1LL << 30),
+  const int64_t w_row = ((d->ld_w_in > d->width ? d->ld_w_in : d->width) + 63) / 64 * 64;  // (the longer row if it is packed)
+  CRADLE_CHECK_ARG(((int64_t)d->hidden + 64 + 256) * w_row < (1LL << 30),
                    "%s: hidden x ld(w_in) must stay below 2^30 elements", what);
   CRADLE_CHECK_ARG(d->ld_x >= d->width && d->ld_w_in >= d->width && d->ld_w_out >= d->hidden, "%s: leading dimension below the row length", what);
   CRADLE_CHECK_ARG(d->ld_x < (1 << 22) && d->ld_w_in < (1 << 22) && d->ld_w_out < (1 << 22) && d->ld_dy < (1 << 22),
@@ -179,6 +187,7 @@ int cradle_gated_mlp_fwd(const cradle_gated_mlp_desc* d, cradle_stream_t s) {
   const Plan p = plan_of(d);
   if (few_rows(d)) {
     if (p.M == 1) few_rows_by_type<1>(d, p, s);
+    else if (d->rows <= kFewRows / 2) few_rows_by_type<kFewRows / 2>(d, p, s);
     else few_rows_by_type<kFewRows>(d, p, s);
   } else {
     forward_of(d, p, s, true);

@@ -160,3 +160,24 @@ def test_repeats_bit_for_bit():
 def test_blocks_too_large_for_a_second_plane(dtype, bias):
     # rows * hidden * (width + out) >= 2^28: h and [dg | du] in the tensors' type; no extent a multiple of a tile
     _check(*_inputs(700, 633, 611, 592, dtype, bias=bias), act="gelu" if bias else "silu")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_rows_of_unaligned_widths(dtype):
+    # from 2048 rows on 16-bit operands whose rows do not start on cache lines are packed, and the hidden axis is padded to 64
+    _check(*_inputs(2050, 200, 1032, 136, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dot_products_and_tiles_for_a_few_rows(dtype):
+    # both sides of the rows where the tile products take over, for small and for large weights
+    for rows in (3, 4, 5, 8, 9):
+        x, w_in, w_out, b_in, b_out, _ = _inputs(rows, 72, 100, 64, dtype, seed=rows)
+        want, _ = ref.gated_mlp(x, w_in, w_out, b_in, b_out, torch.zeros(rows, 64, dtype=dtype), "silu", None)
+        y = ops.gated_mlp(x.cuda(), w_in.cuda(), w_out.cuda(), b_in.cuda(), b_out.cuda())
+        ref.close(y, want["y"][0], want["y"][1], f"{rows} rows")
+    x, w_in, w_out, b_in, b_out, _ = _inputs(5, 2048, 2816, 2048, dtype)  # 2816 x 6144 >= 2^24 weights
+    want, _ = ref.gated_mlp(x, w_in, w_out, b_in, b_out, torch.zeros(5, 2048, dtype=dtype), "silu", None)
+    for rows in (4, 5):
+        y = ops.gated_mlp(x[:rows].cuda(), w_in.cuda(), w_out.cuda(), b_in.cuda(), b_out.cuda())
+        ref.close(y, want["y"][0][:rows], want["y"][1][:rows], f"{rows} rows, large weights")
