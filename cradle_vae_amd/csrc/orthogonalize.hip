@@ -446,13 +446,14 @@ bool small_fits(int m, int n) { return (m <= 128 && n <= 128) || (m <= 64 && n <
 inline int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 
 // Square tiles of 256, 192, 128 and 64 (the 192-wide ones only for the symmetric products: their 192 rows do not fit the
-// MN-major staging).  One workgroup per CU, two of the smallest.
+// MN-major staging).  One workgroup per CU, two of the smallest.  The 128-wide tile has eight waves and four stages: short sums are
+// bound by the loads' latency (2048 x 2048 x 512 on two planes: 15.7 us, with four waves and two longer stages 17.8).
 template <bool BK, int NPL>
 struct Tiles {
   static constexpr int K = NPL == 1 ? 64 : 32;
   using T256 = Tile<F16, NPL, NPL, 256, 256, K, 2, 2, 4, true, BK>;
   using T192 = Tile<F16, NPL, NPL, 192, 192, K, 3, 2, 2, true, true>;
-  using T128 = Tile<F16, NPL, NPL, 128, 128, 64, 2, 2, 2, true, BK>;
+  using T128 = Tile<F16, NPL, NPL, 128, 128, K, 4, 2, 4, true, BK>;
   using T64 = Tile<F16, NPL, NPL, 64, 64, 64, 2, 2, 2, true, BK>;
   using T64Deep = Tile<F16, NPL, NPL, 64, 64, 64, 4, 2, 2, true, BK>;
 };

@@ -451,7 +451,8 @@ def _rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
 
 
 def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    ld, (rows, cols) = t.stride(0), t.shape
+    return ld if rows > 1 or ld > cols else cols
 
 
 def _same_place(what: str, ref: torch.Tensor, **others) -> None:
@@ -491,20 +492,13 @@ class _on:
             self.guard.__exit__(*exc)
 
 
-def _norm_params(what: str, x: torch.Tensor, **params) -> Tuple[list, torch.dtype]:
-    """The parameter vectors of a norm over x's last axis, checked, and their common type (x's own without any)."""
-    out, dtype = [], None
-    for name, t in params.items():
-        if t is not None:
-            if (t.dtype is not x.dtype and t.dtype is not torch.float32) or t.dim() != 1 or t.shape[0] != x.shape[-1]:
-                raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, expected ({x.shape[-1]},) of {x.dtype} or fp32")
-            if dtype is not None and t.dtype is not dtype:
-                raise hip.CradleHipError(f"{what}: {name} is {t.dtype} beside {dtype}")
-            if t.get_device() != x.get_device():
-                raise hip.CradleHipError(f"{what}: {name} is on {t.device}, x on {x.device}")
-            dtype, t = t.dtype, t if t.is_contiguous() else t.contiguous()
-        out.append(t)
-    return out, dtype if dtype is not None else x.dtype
+def _norm_param(what: str, name: str, t: torch.Tensor, D: int, dtype: torch.dtype, device: int) -> torch.Tensor:
+    """A parameter vector of a norm over D numbers of type ``dtype``, checked, contiguous."""
+    if (t.dtype is not dtype and t.dtype is not torch.float32) or t.dim() != 1 or t.numel() != D:
+        raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, expected ({D},) of {dtype} or fp32")
+    if t.get_device() != device:
+        raise hip.CradleHipError(f"{what}: {name} is on {t.device}, x on device {device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
@@ -512,16 +506,23 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``layer_norm_bwd`` reads.  ``x`` fp32 / bf16 / fp16, rows may be strided; ``weight`` / ``bias`` of x's type or fp32
     (``cradle_layer_norm_fwd``)."""
     x2 = _rows_of(x, "layer_norm")
-    (weight, bias), w_dtype = _norm_params("layer_norm", x, weight=weight, bias=bias)
     rows, D = x2.shape
-    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
-    stats = x.new_empty((2, rows), dtype=torch.float32)
-    at = stats.data_ptr()
+    dtype = w_dtype = x.dtype
+    if weight is not None:
+        weight = _norm_param("layer_norm", "weight", weight, D, dtype, x.get_device())
+        w_dtype = weight.dtype
+    if bias is not None:
+        bias = _norm_param("layer_norm", "bias", bias, D, dtype, x.get_device())
+        if weight is not None and bias.dtype is not w_dtype:
+            raise hip.CradleHipError(f"layer_norm: bias is {bias.dtype} beside {w_dtype}")
+        w_dtype = bias.dtype
+    y = torch.empty_like(x) if x2 is x and x.is_contiguous() else x.new_empty(x.shape)
+    stats = x.shape[:-1] if x.dim() != 2 else rows
+    mean, rstd = x.new_empty(stats, dtype=torch.float32), x.new_empty(stats, dtype=torch.float32)
     with _on(x) as s:
         hip.check(hip.load().cradle_layer_norm_fwd(
-            x2.data_ptr(), _ld(x2), _pointer(weight), _pointer(bias), FLOAT_TYPES[x.dtype], FLOAT_TYPES[w_dtype], eps, y.data_ptr(), D,
-            at, at + 4 * rows, rows, D, s), "layer_norm_fwd")
-    mean, rstd = (stats if x.dim() == 2 else stats.reshape(2, *x.shape[:-1])).unbind(0)
+            x2.data_ptr(), _ld(x2), _pointer(weight), _pointer(bias), FLOAT_TYPES[dtype], FLOAT_TYPES[w_dtype], eps, y.data_ptr(), D,
+            mean.data_ptr(), rstd.data_ptr(), rows, D, s), "layer_norm_fwd")
     return y, mean, rstd
 
 
@@ -533,34 +534,33 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise hip.CradleHipError(f"{what}: dy is {dy.dtype} {tuple(dy.shape)} on {dy.device}, x {x.dtype} {tuple(x.shape)} on {x.device}")
     x2, dy2 = _rows_of(x, what), _rows_of(dy, what)
-    (weight,), p_dtype = _norm_params(what, x, weight=weight)
-    if weight is None and param_dtype is not None:
-        p_dtype = param_dtype
-        if p_dtype is not x.dtype and p_dtype is not torch.float32:
-            raise hip.CradleHipError(f"{what}: param_dtype {p_dtype} is neither x's type nor fp32")
     rows, D = x2.shape
+    dtype = p_dtype = x.dtype
+    if weight is not None:
+        weight = _norm_param(what, "weight", weight, D, dtype, x.get_device())
+        p_dtype = weight.dtype
+    elif param_dtype is not None:
+        p_dtype = param_dtype
+        if p_dtype is not dtype and p_dtype is not torch.float32:
+            raise hip.CradleHipError(f"{what}: param_dtype {p_dtype} is neither x's type nor fp32")
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype is not torch.float32 or t.numel() != rows or t.get_device() != x.get_device() or not t.is_contiguous():
             raise hip.CradleHipError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, expected {rows} contiguous fp32 numbers on {x.device}")
-    dx = None if not need_dx else torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
-    dw = db = ws = at = at_w = at_b = None
+    dx = None if not need_dx else torch.empty_like(x) if x2 is x and x.is_contiguous() else x.new_empty(x.shape)
+    dw = db = ws = None
     if rows == 0:
         if need_params:
             dw, db = x.new_zeros((2, D), dtype=p_dtype).unbind(0)
         return dx, dw, db
     lib, need = hip.load(), 0
     if need_params:
-        grads = x.new_empty((2, D), dtype=p_dtype)
-        at_w = grads.data_ptr()
-        at_b = at_w + D * grads.element_size()
-        dw, db = grads.unbind(0)
+        dw, db = x.new_empty(D, dtype=p_dtype), x.new_empty(D, dtype=p_dtype)
         need = lib.cradle_layer_norm_workspace_floats(rows, D)
-        ws = x.new_empty((need,), dtype=torch.float32)
-        at = ws.data_ptr()
+        ws = x.new_empty(need, dtype=torch.float32)
     with _on(x) as s:
         hip.check(lib.cradle_layer_norm_bwd(
             dy2.data_ptr(), _ld(dy2), x2.data_ptr(), _ld(x2), _pointer(weight), mean.data_ptr(), rstd.data_ptr(),
-            FLOAT_TYPES[x.dtype], FLOAT_TYPES[p_dtype], _pointer(dx), D, at_w, at_b, at, need, rows, D, s), what)
+            FLOAT_TYPES[dtype], FLOAT_TYPES[p_dtype], _pointer(dx), D, _pointer(dw), _pointer(db), _pointer(ws), need, rows, D, s), what)
     return dx, dw, db
 
 
