@@ -88,3 +88,17 @@ def test_scales_zeros_and_what_is_not_finite():
     assert bool(torch.isnan(got[0]).any()) and torch.equal(got[1], base[0])
     assert ops.orthogonalize(torch.empty(0, 4, 5, device="cuda")).shape == (0, 4, 5)
     assert ops.orthogonalize(torch.empty(3, 0, 5, device="cuda")).shape == (3, 0, 5)
+
+
+@pytest.mark.parametrize("m,n", [(48, 72), (200, 144)])
+def test_result_over_a_part_of_the_input(m, n):
+    # out starts one matrix further on in the same buffer (small matrices: one workgroup each; larger ones: several launches)
+    g = _matrix(4, m, n, torch.float32)
+    want = ops.orthogonalize(g[:3].cuda())
+    buf = g.cuda()
+    assert torch.equal(ops.orthogonalize(buf[:3], out=buf[1:]), want)
+    buf = g.cuda()
+    rows = buf.reshape(4 * m, n)[::2].reshape(2, m, n)  # every second row of what out begins with
+    want = ops.orthogonalize(rows.clone())
+    view = buf.reshape(4 * m, n).as_strided((2, m, n), (2 * m * n, 2 * n, 1))
+    assert torch.equal(ops.orthogonalize(view, out=buf[:2]), want)
