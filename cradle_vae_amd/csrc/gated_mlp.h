@@ -145,7 +145,7 @@ template <int ELEM, int NPH>
 struct GateEpi {
   static constexpr bool PAIR = true;
   using State = Four;  // the bias of this lane's columns
-  int act, hidden, hidden_p;  // hidden_p: hidden rounded up to 8
+  int act, hidden, hidden_p;  // hidden_p: row length of h, the padding zero
   int dtype;
   const void* bias;  // (2 hidden) or NULL
   u16* h;

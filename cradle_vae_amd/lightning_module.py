@@ -76,6 +76,8 @@ class PerturbationLightningModule(_Base):
         super().__init__()
         if optimizer not in OPTIMIZERS:
             raise ValueError(f"optimizer={optimizer!r}: expected one of {OPTIMIZERS}")
+        if use_scheduler and optimizer != "adam":  # (the scheduler brings its own SGD: configure_optimizers)
+            raise ValueError(f"optimizer={optimizer!r} with use_scheduler=True: the scheduler's SGD would take its place")
         self.optimizer_name = optimizer
         self.loss_module = loss_module
         self.lr = lr

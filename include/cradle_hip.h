@@ -425,7 +425,7 @@ enum { CRADLE_F32 = 0, CRADLE_BF16 = 1, CRADLE_F16 = 2 };
 
 /* Layer norm over the last axis: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), var the mean squared
  * deviation.  x (rows, width), y (rows, width); weight, bias (width) of type w_dtype (dtype or CRADLE_F32), NULL = 1 / 0;
- * mean, rstd (rows) fp32, NULL = not kept.  1 <= width <= 32768. */
+ * mean, rstd (rows) fp32, NULL = not kept.  1 <= width <= 32768.  Outputs overlap no input, here and in the backward pass. */
 int cradle_layer_norm_fwd(const void* x, int64_t ld_x, const void* weight, const void* bias, int dtype, int w_dtype, float eps,
                           void* y, int64_t ld_y, float* mean, float* rstd, int64_t rows, int width, cradle_stream_t stream);
 /* Backward: dx (rows, width) or NULL; dweight, dbias (width, w_dtype) or NULL -- sums over the rows in a fixed order
@@ -446,7 +446,8 @@ int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
  * blocks, rows * hidden * (width + out_width) < 2^28: to twice their bits).  fp32 inputs of
  * magnitude above 3.39e38 count as infinite.  workspace: cradle_gated_mlp_workspace_bytes(desc, backward) bytes, 16-byte aligned;
  * only the sizes, types, pointers' alignment and which pointers are NULL are read for it.
- * hidden * ld_w_in < 2^30, widths <= 2^20, leading dimensions < 2^22. */
+ * (hidden + 320) * ld_w_in (rounded up to 64) < 2^30, widths <= 2^20, leading dimensions < 2^22.  No output may overlap an input or
+ * another output, but y may be the residual. */
 typedef struct cradle_gated_mlp_desc {
   int rows, width, hidden, out_width, dtype, act;
   const void* x; int64_t ld_x;
@@ -477,7 +478,7 @@ int cradle_gated_mlp_bwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stre
  * smaller side); out = X.  g, out: CRADLE_F32 / BF16 / F16, rows contiguous, leading dimensions and batch strides in elements.
  * fp32 accuracy throughout, one rounding to the output's type.  The polynomial s -> a s + b s^3 + c s^5, iterated from [0, 1],
  * has to stay below 8 in magnitude together with b s^2 + c s^4 (the caller checks its coefficients; beyond 16 entries may
- * overflow to infinity).  out may be g.  workspace: cradle_orthogonalize_workspace_bytes bytes, 16-byte aligned. */
+ * overflow to infinity).  out may be g itself, not overlap it otherwise.  workspace: cradle_orthogonalize_workspace_bytes bytes, 16-byte aligned. */
 int64_t cradle_orthogonalize_workspace_bytes(int batch, int m, int n);
 int cradle_orthogonalize(const void* g, int64_t ld_g, int64_t batch_stride_g, void* out, int64_t ld_out, int64_t batch_stride_out,
                          int dtype, int batch, int m, int n, int steps, float a, float b, float c, float eps, void* workspace,

@@ -145,3 +145,13 @@ def test_default_configuration_is_untouched():
     mod = _module(gio.load_elbo("tiny"))
     assert type(mod.configure_optimizers()) is torch.optim.Adam and mod.optimizer_name == "adam"
     assert not any("w_in" in k or "norm." in k for k in mod.state_dict())
+
+
+def test_an_optimizer_that_a_scheduler_would_replace_is_refused():
+    from cradle_vae_amd.lightning_module import PerturbationLightningModule
+
+    kwargs = dict(loss_module=torch.nn.Linear(2, 2), lr=1e-3, n_treatments=2, n_qc=2)
+    with pytest.raises(ValueError, match="use_scheduler"):
+        PerturbationLightningModule(**kwargs, optimizer="muon", use_scheduler=True)
+    assert PerturbationLightningModule(**kwargs, optimizer="muon").optimizer_name == "muon"
+    assert PerturbationLightningModule(**kwargs, use_scheduler=True).use_scheduler
