@@ -16,6 +16,8 @@
 // bound by the matrix cores and the epilogues that a 256 x 256 tile, alone on its CU, does not hide; 1537 rows, 1000 x 2731 in fp16
 // 217 us and 2560 rows, 400 x 800 in fp32 186 us, bound by the loads' latency over sums of 13 to 43 K tiles.
 #pragma once
+#include <type_traits>
+
 #include "mm16.h"
 
 namespace cradle {
@@ -288,7 +290,7 @@ struct PartialEpi {
   __device__ __forceinline__ NoState begin(int, int) const { return {}; }
   template <class T>
   __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, NoState&, int, int) const {
-    float* base = partial + (int64_t)blockIdx.z * a.M * Np;
+    float* base = partial + (int64_t)a.split * a.M * Np;
     each_piece<T, T::WN>(buf, lane, [&](int r, int c, const f32x4* p) {
       const int m = m0 + r, n = n0 + c;
       if (m < a.M && n < a.N) *reinterpret_cast<f32x4*>(base + (int64_t)m * Np + n) = *p;
@@ -521,29 +523,121 @@ int splits_of(const Args& a) {
   return (int)(want < most ? want : most);
 }
 
-// the product into its tensor, or into partial sums that `finish` joins
+// A product's result into its tensor, or, split along K, into partial sums (splits, M, Np) that `finish` joins.
+struct EitherEpi {
+  static constexpr bool PAIR = false;
+  using State = Four;
+  OutEpi out;
+  PartialEpi partial;
+  template <class T>
+  __device__ __forceinline__ Four begin(int n0, int lane) const { return out.begin<T>(n0, lane); }
+  template <class T>
+  __device__ __forceinline__ void emit(const Args& a, float* buf, int m0, int n0, int lane, const Four& b, int tm, int tn) const {
+    NoState none;
+    if (partial.partial) partial.emit<T>(a, buf, m0, n0, lane, none, tm, tn);
+    else out.emit<T>(a, buf, m0, n0, lane, b, tm, tn);
+  }
+  template <class T>
+  __device__ __forceinline__ void finish(const Args&, int, int, const Four&, int, int) const {}
+};
+
+// Independent products of small tiles in one launch, of up to three types of tiles: the backward pass's last three.  Each alone
+// fills the chip about once, with a start and an end at which much of it waits: 2560 rows, 400 x 800 in fp32 81 us in three
+// launches, 67 in one; 1537 rows, 1000 x 2731 in fp16 82 and 67.
+struct Products {
+  Args a[3];
+  EitherEpi e[3];
+  int tiles[3] = {0, 0, 0}, first[3] = {0, 0, 0}, blocks = 0;
+};
+template <class T0, class T1, class T2>
+__global__ __launch_bounds__(256, 2) void products_kernel(const Products p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  static_assert(T0::NT == 256 && T1::NT == 256 && T2::NT == 256 && T0::STAGES == 2 && T1::STAGES == 2 && T2::STAGES == 2, "small tiles");
+  constexpr int A = T0::STAGE > T1::STAGE ? T0::STAGE : T1::STAGE, STAGE = A > T2::STAGE ? A : T2::STAGE;
+  __shared__ u32x4 st0[STAGE];
+  __shared__ u32x4 st1[STAGE];
+  const int k = (int)blockIdx.x >= p.first[2] ? 2 : (int)blockIdx.x >= p.first[1] ? 1 : 0, block = blockIdx.x - p.first[k];
+  Args a = p.a[k];
+  a.split = block / p.tiles[k];
+  const int wg = block % p.tiles[k];
+  if (k == 0) {
+    product_body<T0, EitherEpi>(a, p.e[0], wg, p.tiles[0], st0, st1, nullptr, nullptr);
+  } else if constexpr (std::is_same_v<T1, T2>) {
+    product_body<T1, EitherEpi>(a, p.e[k], wg, p.tiles[k], st0, st1, nullptr, nullptr);
+  } else if (k == 1) {
+    product_body<T1, EitherEpi>(a, p.e[1], wg, p.tiles[1], st0, st1, nullptr, nullptr);
+  } else {
+    product_body<T2, EitherEpi>(a, p.e[2], wg, p.tiles[2], st0, st1, nullptr, nullptr);
+  }
+#endif
+}
+
+// shares that a split along K comes to (every share has work), and the joining of their sums
+template <class T>
+int shares_of(Args& a, int splits) {
+  const int k_tiles = (a.K + T::BK - 1) / T::BK;
+  a.k_tiles_per_split = (k_tiles + splits - 1) / splits;
+  return (k_tiles + a.k_tiles_per_split - 1) / a.k_tiles_per_split;
+}
+inline PartialEpi split_product(const Args& a, const OutEpi& epi, float* partial, int shares, Finish& finish) {
+  FinishJob j{};
+  j.partial = partial, j.n = shares, j.ld = (a.N + 3) & ~3, j.M = a.M, j.out = epi;
+  const int64_t blocks = ((int64_t)a.M * (j.ld / 4) + 255) / 256;
+  finish.add(j, blocks < 1024 ? blocks : 1024);
+  return PartialEpi{partial, j.ld};
+}
+
+// A product into its tensor
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
-void product_out(const Args& a, const OutEpi& epi, float* partial, Finish& finish, hipStream_t s) {
+void product_out(Args a, const OutEpi& epi, float* partial, Finish& finish, hipStream_t s) {
   const int splits = splits_of<ELEM, NPA, NPB, AK, BK>(a);
   if (splits == 1) return product<ELEM, NPA, NPB, AK, BK>(a, epi, a.N, s);
   using Small = typename Tiles<ELEM, NPA, NPB, AK, BK>::Small;
-  const int Np = (a.N + 3) & ~3;
-  const int k_tiles = (a.K + Small::BK - 1) / Small::BK, per = (k_tiles + splits - 1) / splits;
-  const int used = (k_tiles + per - 1) / per;  // (every share has work)
-  launch<Small>(a, PartialEpi{partial, Np}, a.N, used, s);
-  FinishJob j{};
-  j.partial = partial, j.n = used, j.ld = Np, j.M = a.M, j.out = epi;
-  const int64_t blocks = ((int64_t)a.M * (Np / 4) + 255) / 256;
-  finish.add(j, blocks < 1024 ? blocks : 1024);
+  const int shares = shares_of<Small>(a, splits);
+  launch<Small>(a, split_product(a, epi, partial, shares, finish), a.N, shares, s);
+}
+// the same, at once with large tiles (splits == 0), else as the k-th of `ps`
+template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+void product_out(Args a, const OutEpi& epi, int splits, float* partial, Products& ps, int k, Finish& finish, hipStream_t s) {
+  using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
+  using Small = typename TT::Small;
+  if (!splits) return launch<typename TT::Large>(a, epi, a.N, 1, s);
+  const int shares = shares_of<Small>(a, splits);
+  a.tiles_m = (a.M + Small::BM - 1) / Small::BM;
+  a.tiles_n = (a.N + Small::BN - 1) / Small::BN;
+  a.symmetric = 0;
+  ps.a[k] = a;
+  ps.e[k] = EitherEpi{epi, splits > 1 ? split_product(a, epi, partial, shares, finish) : PartialEpi{}};
+  ps.tiles[k] = a.tiles_m * a.tiles_n;
+  ps.blocks += ps.tiles[k] * shares;
+}
+template <class T0, class T1, class T2>
+void run_products(const Products& p, hipStream_t s) {
+  if (p.blocks) hipLaunchKernelGGL((products_kernel<T0, T1, T2>), dim3((unsigned)p.blocks), dim3(256), 0, s, p);
 }
 
-template <int ELEM, int NPA, int NPB, bool AK, bool BK>
-int64_t partial_floats(int M, int N, int K) {
-  Args a{};
-  a.M = M, a.N = N, a.K = K;
-  const int s = splits_of<ELEM, NPA, NPB, AK, BK>(a);
-  return s == 1 ? 0 : (int64_t)s * M * ((N + 3) & ~3);
-}
+inline int64_t partial_floats(const Args& a, int splits) { return splits < 2 ? 0 : (int64_t)splits * a.M * ((a.N + 3) & ~3); }
+
+// Splits along K of products that share a launch: shares of about equal length, 0.7 of what each of the 2 kCUs places gets in
+// all -- shorter ones cost more partial sums, longer ones leave places idle at the end (both passes of 8192 rows, 512 x 1024 in fp32
+// with 0.5 556 us, 0.7 536, 1.4 616; 4096 rows in bf16 126, 125, 118).  0: large tiles are faster.
+struct Splits {
+  double work = 0;  // K tiles of all small tiles
+  template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+  int of(const Args& a) const {
+    using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
+    if (use_large<typename TT::Large, typename TT::Small>(a, a.N, false)) return 0;
+    const int k_tiles = (a.K + TT::Small::BK - 1) / TT::Small::BK, most = k_tiles / 4;
+    const int n = (int)(k_tiles * (2 * kCUs / 0.7) / work + 0.5);
+    return n < 1 || most < 1 ? 1 : n < most ? n : most;
+  }
+  template <int ELEM, int NPA, int NPB, bool AK, bool BK>
+  void add(const Args& a) {
+    using TT = Tiles<ELEM, NPA, NPB, AK, BK>;
+    if (use_large<typename TT::Large, typename TT::Small>(a, a.N, false)) return;
+    work += (double)tiles<typename TT::Small>(a, a.N, false) * ((a.K + TT::Small::BK - 1) / TT::Small::BK);
+  }
+};
 
 inline int vec_ok(const void* p, int64_t ld, int dtype) { return ld % 4 == 0 && ((uintptr_t)p & (dtype == CRADLE_F32 ? 15 : 7)) == 0; }
 constexpr int kNoGap = 0x7fffffff;
@@ -565,8 +659,9 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, p.M, ws, js, n);
   const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, p.M, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp;
+  const Args out_args = args_of({}, w_out, p.M, p.O, p.Fp);
   u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * NPH * 2));
-  float* partial = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, true>(p.M, p.O, p.Fp) * 4));
+  float* partial = static_cast<float*>(ws.take(partial_floats(out_args, splits_of<ELEM, NPH, NPL, true, true>(out_args)) * 4));
   if (!run) return ws.off;
   run_pack<ELEM, NPL>(p, js, n, s);
   Args a = args_of(x, w_in, p.M, p.F, p.K);
@@ -601,9 +696,18 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   const Operand dy = operand(p, d->dy, d->ld_dy, p.M, p.O, p.M, kNoGap, 0, p.F, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp, d_plane = 2 * h_plane;
   u16* dgu = static_cast<u16*>(ws.take(d_plane * NPH * 2));
-  float* p_dx = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, true, false>(p.M, p.K, 2 * p.Fp) * 4));
-  float* p_in = static_cast<float*>(ws.take(partial_floats<ELEM, NPH, NPL, false, false>(2 * p.Fp, p.K, p.M) * 4));
-  float* p_out = static_cast<float*>(ws.take(partial_floats<ELEM, NPL, NPH, false, false>(p.O, p.F, p.M) * 4));
+  const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
+  const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};
+  const Args dx = args_of(dop, w_in, p.M, p.K, 2 * p.Fp), dw_in = args_of(dop, x, 2 * p.Fp, p.K, p.M), dw_out = args_of(dy, hop, p.O, p.F, p.M);
+  Splits sp;
+  if (d->dx) sp.add<ELEM, NPH, NPL, true, false>(dx);
+  if (d->dw_in) sp.add<ELEM, NPH, NPL, false, false>(dw_in);
+  if (d->dw_out) sp.add<ELEM, NPL, NPH, false, false>(dw_out);
+  const int n_dx = d->dx ? sp.of<ELEM, NPH, NPL, true, false>(dx) : 0, n_in = d->dw_in ? sp.of<ELEM, NPH, NPL, false, false>(dw_in) : 0,
+            n_out = d->dw_out ? sp.of<ELEM, NPL, NPH, false, false>(dw_out) : 0;
+  float* p_dx = static_cast<float*>(ws.take(partial_floats(dx, n_dx) * 4));
+  float* p_in = static_cast<float*>(ws.take(partial_floats(dw_in, n_in) * 4));
+  float* p_out = static_cast<float*>(ws.take(partial_floats(dw_out, n_out) * 4));
   const int sum_rows = (p.M + 127) / 128 * 4;  // of either tile size: 128 rows are at most four wave rows
   float* sums = static_cast<float*>(ws.take(d->db_in ? (int64_t)sum_rows * 2 * p.Fp * 4 : 0));
   const int per = colsum_rows(p.M), shares = (p.M + per - 1) / per;
@@ -626,14 +730,17 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
     hipLaunchKernelGGL(colsum_kernel<DT>, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.M, p.O, per, sums_out);
     add_column_sums(finish, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
   }
-  const Operand dop{dgu, 2 * (int64_t)p.Fp, d_plane, 0};
-  const Operand hop{static_cast<const u16*>(d->saved_h), p.Fp, h_plane, 0};
   auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g, int cols) {
     return OutEpi{q, ld, p.dtype, nullptr, nullptr, 0, rows, gap_at, g, cols, vec_ok(q, ld, p.dtype)};
   };
-  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(args_of(dop, w_in, p.M, p.K, 2 * p.Fp), out(d->dx, d->ld_dx, p.M, kNoGap, 0, p.K), p_dx, finish, s);
-  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(args_of(dop, x, 2 * p.Fp, p.K, p.M), out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), p_in, finish, s);
-  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(args_of(dy, hop, p.O, p.F, p.M), out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), p_out, finish, s);
+  Products ps;
+  if (d->dx) product_out<ELEM, NPH, NPL, true, false>(dx, out(d->dx, d->ld_dx, p.M, kNoGap, 0, p.K), n_dx, p_dx, ps, 0, finish, s);
+  ps.first[1] = ps.blocks;
+  if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(dw_in, out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), n_in, p_in, ps, 1, finish, s);
+  ps.first[2] = ps.blocks;
+  if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(dw_out, out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), n_out, p_out, ps, 2, finish, s);
+  run_products<typename Tiles<ELEM, NPH, NPL, true, false>::Small, typename Tiles<ELEM, NPH, NPL, false, false>::Small,
+               typename Tiles<ELEM, NPL, NPH, false, false>::Small>(ps, s);
   run_finish(finish, s);
   return ws.off;
 }

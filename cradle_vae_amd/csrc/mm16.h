@@ -95,7 +95,8 @@ struct Args {
   int M, N, K;           // N: columns of the output (for a paired product: of each half)
   int tiles_m, tiles_n;
   int up_row;            // paired product: rows of B from here on are the second half
-  int k_tiles_per_split; // blockIdx.z-th share of the K tiles
+  int k_tiles_per_split; // K tiles of a share
+  int split;             // this workgroup's share (set in the kernel)
   int symmetric;         // 1: only the tiles on and below the diagonal are computed (square tiles, tiles_m == tiles_n)
 };
 
@@ -240,9 +241,7 @@ struct PairMap {
 
 // Order of the tiles: workgroups go round-robin over the eight XCDs, so the tiles of one XCD (its own L2) are a contiguous
 // run of a raster of 8 tile rows at a time.
-__device__ __forceinline__ void tile_of(const Args& a, int& tm, int& tn) {
-  const int nwg = gridDim.x;
-  int wg = blockIdx.x;
+__device__ __forceinline__ void tile_of(const Args& a, int wg, int nwg, int& tm, int& tn) {
   const int q = nwg / 8, r = nwg % 8, xcd = wg % 8, pos = wg / 8;
   wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + pos;
   if (a.symmetric) {  // tile rows' lengths are 1, 2, 3 ...
@@ -312,19 +311,16 @@ __device__ __forceinline__ void each_turned_piece(const float* buf, int lane, co
 // Epi: begin(n0, lane) once -> state (a lane's column does not change), emit(a, buf, m0, n0, lane, state, tm, tn) for every 32 rows,
 // finish(...) once; Epi::PAIR: columns [0, WN / 2) of buf are the
 // first half's, [WN / 2, WN) the second's.
+// wg of nwg: this workgroup among those of its share; st0.. : the stages (of at least T::STAGE pieces, as many as T has).
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass only needs the launch stubs; with the body it leaves some of them out)
 template <class T, class Epi>
-__global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const Epi epi) {
-#ifdef __HIP_DEVICE_COMPILE__  // (the host pass only needs the launch stub; with the body it leaves some of them out)
+__device__ __forceinline__ void product_body(const Args& a, const Epi& epi, int wg, int nwg, u32x4* st0, u32x4* st1, u32x4* st2, u32x4* st3) {
   static_assert(!Epi::PAIR || T::TN % 2 == 0, "a wave holds both halves of a column");
   using SA = Stager<T, T::A_KMAJOR, T::BM, T::NPA>;
   using SB = Stager<T, T::B_KMAJOR, T::BN, T::NPB>;
   constexpr int S = T::STAGES;
-  __shared__ u32x4 st0[T::STAGE];
-  __shared__ u32x4 st1[T::STAGE];
-  __shared__ u32x4 st2[S > 2 ? T::STAGE : 1];
-  __shared__ u32x4 st3[S > 3 ? T::STAGE : 1];
   int tm, tn;
-  tile_of(a, tm, tn);
+  tile_of(a, wg, nwg, tm, tn);
   const int row0 = tm * T::BM, col0 = tn * (Epi::PAIR ? T::BN / 2 : T::BN);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WAVES_N, wn = wave % T::WAVES_N;
@@ -335,7 +331,7 @@ __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const E
   else sb.init(a.B, col0, a.N, a.K, PlainMap{});
 
   const int k_tiles = (a.K + T::BK - 1) / T::BK;
-  const int kt0 = blockIdx.z * a.k_tiles_per_split, kt1 = min(k_tiles, kt0 + a.k_tiles_per_split);
+  const int kt0 = a.split * a.k_tiles_per_split, kt1 = min(k_tiles, kt0 + a.k_tiles_per_split);
 
   // Where the registers allow, the products of lower planes are summed apart: in one accumulator each of them would be rounded
   // at the size of the whole sum (six roundings per 16 of K instead of one).
@@ -494,6 +490,20 @@ __global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args a, const E
     wave_sync();
   }
   epi.template finish<T>(a, n0, lane, state, tm, wm);
+}
+#endif
+
+// one product: blockIdx.x the tile, y the matrix of a batch, z the share of K
+template <class T, class Epi>
+__global__ __launch_bounds__(T::NT, 1) void product_kernel(const Args args, const Epi epi) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __shared__ u32x4 st0[T::STAGE];
+  __shared__ u32x4 st1[T::STAGE];
+  __shared__ u32x4 st2[T::STAGES > 2 ? T::STAGE : 1];
+  __shared__ u32x4 st3[T::STAGES > 3 ? T::STAGE : 1];
+  Args a = args;
+  a.split = blockIdx.z;
+  product_body<T, Epi>(a, epi, blockIdx.x, gridDim.x, st0, st1, st2, st3);
 #endif
 }
 
