@@ -300,27 +300,37 @@ struct PartialEpi {
   __device__ __forceinline__ void finish(const Args&, int, int, NoState&, int, int) const {}
 };
 
-// column sums in two passes with a fixed order.  First: blockIdx.y-th share of the rows of a (rows, cols) tensor, eight rows'
-// loads in flight per thread.
+// column sums in two passes with a fixed order.  First: shares of rows_per rows of a (rows, cols) tensor, eight rows' loads in flight
+// per thread.
+struct ColumnShares {
+  const void* src;
+  int64_t ld;
+  int rows, cols, rows_per, blocks_n;  // blocks_n: 64 columns each
+  float* partial;
+  int blocks = 0;
+};
 template <int DT>
-static __global__ __launch_bounds__(256) void colsum_kernel(const void* __restrict__ src, int64_t ld, int rows, int cols, int rows_per,
-                                                            float* __restrict__ partial) {
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const int r1 = min(rows, (int)(blockIdx.y + 1) * rows_per);
-  __shared__ float red[4][64];
+__device__ __forceinline__ void column_share(const ColumnShares& j, int block, float (*red)[64]) {
+  const int c = block % j.blocks_n * 64 + (threadIdx.x & 63), share = block / j.blocks_n, w = threadIdx.x >> 6;
+  const int r1 = min(j.rows, (share + 1) * j.rows_per);
   float s = 0.f;
-  if (c < cols)
-    for (int r = blockIdx.y * rows_per + w; r < r1; r += 32) {
+  if (c < j.cols)
+    for (int r = share * j.rows_per + w; r < r1; r += 32) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = r + 4 * k < r1 ? load_as(src, (int64_t)(r + 4 * k) * ld + c, DT) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = r + 4 * k < r1 ? load_as(j.src, (int64_t)(r + 4 * k) * j.ld + c, DT) : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += v[k];
     }
   red[w][threadIdx.x & 63] = s;
   __syncthreads();
-  if (w == 0 && c < cols)
-    partial[(int64_t)blockIdx.y * cols + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+  if (w == 0 && c < j.cols)
+    j.partial[(int64_t)share * j.cols + c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+template <int DT>
+static __global__ __launch_bounds__(256) void column_shares_kernel(const ColumnShares j) {
+  __shared__ float red[4][64];
+  column_share<DT>(j, blockIdx.x, red);
 }
 
 // What is left to do once the products of a pass are done, in one launch: joining products split along K (partial sums in the
@@ -548,6 +558,7 @@ struct Products {
   Args a[3];
   EitherEpi e[3];
   int tiles[3] = {0, 0, 0}, first[3] = {0, 0, 0}, blocks = 0;
+  ColumnShares sums{};  // ride along behind them
 };
 template <class T0, class T1, class T2>
 __global__ __launch_bounds__(256, 2) void products_kernel(const Products p) {
@@ -556,6 +567,10 @@ __global__ __launch_bounds__(256, 2) void products_kernel(const Products p) {
   constexpr int A = T0::STAGE > T1::STAGE ? T0::STAGE : T1::STAGE, STAGE = A > T2::STAGE ? A : T2::STAGE;
   __shared__ u32x4 st0[STAGE];
   __shared__ u32x4 st1[STAGE];
+  if ((int)blockIdx.x >= p.blocks) {
+    constexpr int DT = T0::NPB == 3 ? CRADLE_F32 : T0::ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
+    return column_share<DT>(p.sums, blockIdx.x - p.blocks, reinterpret_cast<float(*)[64]>(st0));
+  }
   const int k = (int)blockIdx.x >= p.first[2] ? 2 : (int)blockIdx.x >= p.first[1] ? 1 : 0, block = blockIdx.x - p.first[k];
   Args a = p.a[k];
   a.split = block / p.tiles[k];
@@ -613,7 +628,7 @@ void product_out(Args a, const OutEpi& epi, int splits, float* partial, Products
 }
 template <class T0, class T1, class T2>
 void run_products(const Products& p, hipStream_t s) {
-  if (p.blocks) hipLaunchKernelGGL((products_kernel<T0, T1, T2>), dim3((unsigned)p.blocks), dim3(256), 0, s, p);
+  if (p.blocks) hipLaunchKernelGGL((products_kernel<T0, T1, T2>), dim3((unsigned)(p.blocks + p.sums.blocks)), dim3(256), 0, s, p);
 }
 
 inline int64_t partial_floats(const Args& a, int splits) { return splits < 2 ? 0 : (int64_t)splits * a.M * ((a.N + 3) & ~3); }
@@ -725,9 +740,9 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
     const int used = large ? (p.M + 255) / 256 * TT::Large::WAVES_M : (p.M + 127) / 128 * TT::Small::WAVES_M;
     add_column_sums(finish, sums, used, 2 * p.Fp, 2 * p.F, p.F, gap, d->db_in, p.dtype);
   }
+  ColumnShares db_out{d->dy, d->ld_dy, p.M, p.O, per, (p.O + 63) / 64, sums_out};
   if (d->db_out) {
-    constexpr int DT = NPL == 3 ? CRADLE_F32 : ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
-    hipLaunchKernelGGL(colsum_kernel<DT>, dim3((p.O + 63) / 64, shares), dim3(256), 0, s, d->dy, d->ld_dy, p.M, p.O, per, sums_out);
+    db_out.blocks = db_out.blocks_n * shares;
     add_column_sums(finish, sums_out, shares, p.O, p.O, kNoGap, 0, d->db_out, p.dtype);
   }
   auto out = [&](void* q, int64_t ld, int rows, int gap_at, int g, int cols) {
@@ -739,6 +754,11 @@ int64_t backward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace,
   if (d->dw_in) product_out<ELEM, NPH, NPL, false, false>(dw_in, out(d->dw_in, p.K, 2 * p.F, p.F, gap, p.K), n_in, p_in, ps, 1, finish, s);
   ps.first[2] = ps.blocks;
   if (d->dw_out) product_out<ELEM, NPL, NPH, false, false>(dw_out, out(d->dw_out, p.F, p.O, kNoGap, 0, p.F), n_out, p_out, ps, 2, finish, s);
+  ps.sums = db_out;
+  if (!ps.blocks && db_out.blocks) {
+    constexpr int DT = NPL == 3 ? CRADLE_F32 : ELEM == BF16 ? CRADLE_BF16 : CRADLE_F16;
+    hipLaunchKernelGGL(column_shares_kernel<DT>, dim3((unsigned)db_out.blocks), dim3(256), 0, s, db_out);
+  }
   run_products<typename Tiles<ELEM, NPH, NPL, true, false>::Small, typename Tiles<ELEM, NPH, NPL, false, false>::Small,
                typename Tiles<ELEM, NPL, NPH, false, false>::Small>(ps, s);
   run_finish(finish, s);

@@ -181,3 +181,16 @@ def test_dot_products_and_tiles_for_a_few_rows(dtype):
     for rows in (4, 5):
         y = ops.gated_mlp(x[:rows].cuda(), w_in.cuda(), w_out.cuda(), b_in.cuda(), b_out.cuda())
         ref.close(y, want["y"][0][:rows], want["y"][1][:rows], f"{rows} rows, large weights")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_weight_gradient_alone(dtype):
+    # a weight gradient of large tiles and nothing beside it: dy's column sums have no other launch to go along with
+    x, w_in, w_out, b_in, b_out, dy = _inputs(70, 4096, 2048, 40, dtype)
+    want, _ = ref.gated_mlp(x, w_in, w_out, b_in, b_out, dy, "silu", None)
+    gx, gi, go = x.cuda(), w_in.cuda(), w_out.cuda()
+    _, saved = ops.gated_mlp(gx, gi, go, b_in.cuda(), b_out.cuda(), save=True)
+    grads = ops.gated_mlp_bwd(dy.cuda(), gx, gi, go, saved, bias=True, need=(False, True, False))
+    assert grads[0] is None and grads[2] is None
+    for i in (1, 3, 4):
+        ref.close(grads[i], want[NAMES[i]][0], want[NAMES[i]][1], NAMES[i])
