@@ -3,7 +3,7 @@
 //   dh = dy W_out,  dg = dh u act'(g),  du = dh act(g)
 //   dx = [dg | du] W_in,  dW_in = [dg | du]^T x,  dW_out = dy^T h,  db_in / db_out: column sums of [dg | du] / dy
 // Two products forward (x W_in^T with both projections, the activation and the gating in its epilogue), four backward (the
-// first with the whole elementwise backward in its epilogue); mm16.h has the tile product and what bounds it.
+// first with the whole elementwise backward in its epilogue, the others in one launch); mm16.h has the tile product and what bounds it.
 //
 // Numbers: bf16 / fp16 tensors multiply as they are; fp32 tensors as three bf16 planes (six products, fp32's accuracy at
 // 2.6x the rate of the fp32 matrix instruction).  Sums, pre-activations and biases are fp32.  h and [dg | du] are inputs of a
@@ -14,7 +14,7 @@
 //
 // Measured, forward and backward: 8192 rows, 4096 x 10240 in bf16 5.2 ms, 1190 TFLOP/s (library products of these sizes: 1290 to 1560),
 // bound by the matrix cores and the epilogues that a 256 x 256 tile, alone on its CU, does not hide; 1537 rows, 1000 x 2731 in fp16
-// 217 us and 2560 rows, 400 x 800 in fp32 186 us, bound by the loads' latency over sums of 13 to 43 K tiles.
+// 193 us and 2560 rows, 400 x 800 in fp32 161 us, bound by the loads' latency over sums of 13 to 30 K tiles.
 #pragma once
 #include <type_traits>
 
@@ -522,7 +522,8 @@ void product(const Args& a, const Epi& epi, int cols, hipStream_t s) {
 }
 
 // A product whose output has too few small tiles for the chip (two per CU at a time) is split along K, into shares of at
-// least four K tiles; its partial sums cost a pass over them, so the large tiles are only left for a real gain.
+// least four K tiles; its partial sums cost a pass over them.  Forward pass, whole and split: 512 rows, 512 x 1024 in fp32 54 and 40 us;
+// 2560 rows, 400 x 800 in fp32 66 and 62; 1537 rows, 1000 x 2731 in fp16 87 and 76; 4096 rows, 512 x 1024 in bf16 38 and 40.
 template <int ELEM, int NPA, int NPB, bool AK, bool BK>
 int splits_of(const Args& a) {
   using TT = Tiles<ELEM, NPA, NPB, AK, BK>;

@@ -13,8 +13,8 @@
 // that of the rounding alone, against up to 1.57 with one plane throughout.
 // S and B are symmetric: only the tiles on and below the diagonal are computed, the epilogue stores them twice.
 // The norm is accumulated in fp64 (squares of fp32 gradients leave fp32's range).
-// Measured, five steps: 4096 x 8192 in bf16 4.46 ms (two-plane steps at 1040 TFLOP/s, one-plane steps at 815: the epilogue that reads
-// and writes both planes of X is not hidden); 5000 x 400 in fp32 211 us, 2 x 513 x 1001 in fp16 193 us: chains of 17 to 22 launches
+// Measured, five steps: 4096 x 8192 in bf16 4.33 ms (two-plane steps at 1040 TFLOP/s, one-plane steps at 815: the epilogue that reads
+// and writes both planes of X is not hidden); 5000 x 400 in fp32 209 us, 2 x 513 x 1001 in fp16 192 us: chains of 17 to 22 launches
 // of 5 to 16 us.
 #include "mm16.h"
 
