@@ -5,6 +5,7 @@ the HIP kernels.  Autograd wiring lives in ``cradle_vae_amd.functional``.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Optional, Tuple
 
@@ -352,7 +353,6 @@ def gemm(
             raise hip.CradleHipError("gemm: extra_col must have M elements")
         d.extra_col = hip.ptr(extra_col)
     ws_ptr, ws_n = (hip.ptr(workspace), workspace.numel()) if workspace is not None else (None, 0)
-    import ctypes
 
     if repeat > 1:
         hip.check(hip.load().cradle_gemm_f32_repeat(ctypes.byref(d), ws_ptr, ws_n, repeat, hip.stream()), "gemm_f32")
@@ -585,13 +585,11 @@ def _gated_desc(what, x, w_in, w_out, act):
     return d, (x2, wi, wo)
 
 
-def _gated_workspace(d, backward: int, device) -> torch.Tensor:
-    import ctypes
-
+def _gated_workspace(d, backward: int, x: torch.Tensor) -> torch.Tensor:
     need = hip.load().cradle_gated_mlp_workspace_bytes(ctypes.byref(d), backward)
     if need < 0:
         hip.check(1, "gated_mlp_workspace_bytes")
-    ws = torch.empty(max(need, 16), device=device, dtype=torch.uint8)
+    ws = x.new_empty(max(need, 16), dtype=torch.uint8)
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
     return ws
 
@@ -602,15 +600,13 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     (2 hidden, width) holds the gate's rows, then the up projection's; ``act`` "silu" or "gelu" (erf); all tensors of one type, fp32 /
     bf16 / fp16 (``cradle_gated_mlp_fwd``).  ``save``: -> (y, saved), what ``gated_mlp_bwd`` reads (the pre-activations in
     fp32 and h); a few rows without ``save`` take the form for single cells, which reads the weights once."""
-    import ctypes
-
     what = "gated_mlp"
     d, keep = _gated_desc(what, x, w_in, w_out, act)
     M, O, F = d.rows, d.out_width, d.hidden
     b_in, b_out = _vector(what, "b_in", b_in, 2 * F, (x.dtype,)), _vector(what, "b_out", b_out, O, (x.dtype,))
     _same_place(what, x, b_in=b_in, b_out=b_out, residual=residual)
     d.b_in, d.b_out = _pointer(b_in), _pointer(b_out)
-    y = torch.empty((*x.shape[:-1], O), device=x.device, dtype=x.dtype)
+    y = x.new_empty((*x.shape[:-1], O))
     d.y, d.ld_y = y.data_ptr(), O
     if residual is not None:
         if residual.shape != y.shape or residual.dtype != x.dtype:
@@ -621,11 +617,11 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     if save:
         hb = ctypes.c_int64()
         gb = lib.cradle_gated_mlp_saved_bytes(M, d.width, F, O, d.dtype, ctypes.byref(hb))
-        saved = (torch.empty(gb // 4, device=x.device, dtype=torch.float32), torch.empty(hb.value // 2, device=x.device, dtype=torch.int16))
+        saved = (x.new_empty(gb // 4, dtype=torch.float32), x.new_empty(hb.value // 2, dtype=torch.int16))
         if M:
             d.saved_gu, d.saved_h = saved[0].data_ptr(), saved[1].data_ptr()
     if M:
-        ws = _gated_workspace(d, 0, x.device)
+        ws = _gated_workspace(d, 0, x)
         with _on(x) as s:
             hip.check(lib.cradle_gated_mlp_fwd(ctypes.byref(d), s), "gated_mlp_fwd")
     return (y, saved) if save else y
@@ -635,8 +631,6 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
                   bias: bool = False, need=(True, True, True)):
     """-> (dx, dw_in, dw_out, db_in, db_out) of ``gated_mlp``; ``need`` says which of the first three are wanted (None in the
     place of the others), ``bias`` whether the biases' gradients are.  The residual's gradient is dy itself."""
-    import ctypes
-
     what = "gated_mlp_bwd"
     d, keep = _gated_desc(what, x, w_in, w_out, act)
     M, K, O, F = d.rows, d.width, d.out_width, d.hidden
@@ -647,17 +641,16 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
     gb = lib.cradle_gated_mlp_saved_bytes(M, d.width, F, O, d.dtype, ctypes.byref(hb))
     if saved[0].numel() * 4 != gb or saved[1].numel() * 2 != hb.value:
         raise hip.CradleHipError(f"{what}: the saved buffers do not belong to a block of these sizes")
-    make = torch.empty if M else torch.zeros
-    new = lambda *shape: make(shape, device=x.device, dtype=x.dtype)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-    dw_in, dw_out = (new(2 * F, K) if need[1] else None), (new(O, F) if need[2] else None)
-    db_in, db_out = (new(2 * F), new(O)) if bias else (None, None)
+    new = x.new_empty if M else x.new_zeros
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw_in, dw_out = (new((2 * F, K)) if need[1] else None), (new((O, F)) if need[2] else None)
+    db_in, db_out = (new((2 * F,)), new((O,))) if bias else (None, None)
     if M:
         dy2 = _rows_of(dy, what)
         d.dy, d.ld_dy, d.saved_gu, d.saved_h = dy2.data_ptr(), _ld(dy2), saved[0].data_ptr(), saved[1].data_ptr()
         d.dx, d.ld_dx, d.dw_in, d.dw_out, d.db_in, d.db_out = (_pointer(dx), K, _pointer(dw_in), _pointer(dw_out), _pointer(db_in),
                                                                _pointer(db_out))
-        ws = _gated_workspace(d, 1, x.device)
+        ws = _gated_workspace(d, 1, x)
         with _on(x) as s:
             hip.check(lib.cradle_gated_mlp_bwd(ctypes.byref(d), s), what)
     return dx, dw_in, dw_out, db_in, db_out
