@@ -214,6 +214,8 @@ def onehot_linear(mask: torch.Tensor, W: torch.Tensor, b: torch.Tensor, t0: int 
 
 # ---------------------------------------------------------------------------------------------
 # normalised, gated hidden layers (no counterpart in the reference's LeakyReLU MLPs)
+# A backward pass captured into a graph: let go of every eager graph over the same leaves before the capture (autograd runs a leaf's
+# accumulation on the stream its node was made on).
 # ---------------------------------------------------------------------------------------------
 class _LayerNorm(torch.autograd.Function):
     @staticmethod

@@ -303,3 +303,57 @@ def test_configured_training_run(tmp_path):
     assert np.isfinite(float(list(csv.DictReader(open(rdir / "metrics.csv")))[-1]["train/loss"]))
     m = eval_entry.main(["--experiment_path", str(rdir), "--batch_size", "64", "--ate_n_particles", "32", "--qc_pass", "false"])
     assert np.isfinite(m["test/IWELBO"])
+
+
+def test_two_calls_at_once():
+    """Independent calls on two streams, each with its own workspace, against the same calls one after the other."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+    x, dy, w_in, w_out, b_in, b_out = n(2, 600, 72), n(2, 600, 72), n(304, 72), n(72, 152), n(304), n(72)
+
+    def work(i):
+        h, mean, rstd = ops.layer_norm(x[i], b_out, b_out)
+        y, saved = ops.gated_mlp(h, w_in, w_out, b_in, b_out, save=True)
+        grads = ops.gated_mlp_bwd(dy[i], h, w_in, w_out, saved, bias=True)
+        return [y, *grads, *ops.layer_norm_bwd(grads[0], x[i], b_out, mean, rstd), ops.orthogonalize(grads[1])]
+
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(work(i))
+        torch.cuda.synchronize()
+        for a, b in zip(got[0] + got[1], want[0] + want[1]):
+            assert torch.equal(a, b)
+
+
+def test_a_captured_backward_pass():
+    """The autograd forms in a captured graph, no eager graph of the same leaves alive at the capture."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+    x, dy = n(90, 40), n(90, 40)
+    leaves = [p.requires_grad_() for p in (n(40), n(40), n(112, 40), n(40, 56), n(112), n(40))]
+
+    def work():
+        w, b, w_in, w_out, b_in, b_out = leaves
+        y = F_hip.gated_mlp(F_hip.layer_norm(x, w, b), w_in, w_out, b_in, b_out, residual=x)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = work()
+    for _ in range(3):
+        x.copy_(n(90, 40))
+        dy.copy_(n(90, 40))
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, work()):
+            assert torch.equal(a, b)
