@@ -665,14 +665,14 @@ def _ns_bound(coeffs, steps: int) -> float:
     a, b, c = (float(v) for v in coeffs)
     if not all(abs(v) < float("inf") for v in (a, b, c)):
         return float("inf")
-    s, most = torch.linspace(0, 1, 4097, dtype=torch.float64), 1.0
+    s, most = torch.linspace(0, 1, 4097, dtype=torch.float64, device="cpu"), 1.0
     for _ in range(steps):
         q = b * s * s + c * s ** 4
         s = a * s + q * s
         most = max(most, float(q.abs().max()), float(s.abs().max()))
         if not most < 1e6:
             return float("inf")
-        s = torch.linspace(0, float(s.abs().max()), 4097, dtype=torch.float64)  # (every value between: a superset)
+        s = torch.linspace(0, float(s.abs().max()), 4097, dtype=torch.float64, device="cpu")  # (every value between: a superset)
     return most
 
 

@@ -155,3 +155,9 @@ def test_an_optimizer_that_a_scheduler_would_replace_is_refused():
         PerturbationLightningModule(**kwargs, optimizer="muon", use_scheduler=True)
     assert PerturbationLightningModule(**kwargs, optimizer="muon").optimizer_name == "muon"
     assert PerturbationLightningModule(**kwargs, use_scheduler=True).use_scheduler
+
+
+def test_the_bound_on_the_coefficients_stays_on_the_host():
+    ops._ns_bound.cache_clear()
+    with torch.device("meta"):  # (a default device: no kernel may be needed to check the arguments)
+        assert 1 < ops._ns_bound(ops.NS_COEFFS, 5) < 8
