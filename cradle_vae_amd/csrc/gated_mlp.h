@@ -675,7 +675,8 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   const Operand w_in = operand(p, d->w_in, d->ld_w_in, 2 * p.F, p.K, 2 * p.Fp, p.F, gap, p.M, ws, js, n);
   const Operand w_out = operand(p, d->w_out, d->ld_w_out, p.O, p.F, p.O, kNoGap, 0, p.M, ws, js, n);
   const int64_t h_plane = (int64_t)p.M * p.Fp;
-  const Args out_args = args_of({}, w_out, p.M, p.O, p.Fp);
+  // (the inner extent is F: of h's padding and of a directly staged W_out's neighbours nothing is multiplied)
+  const Args out_args = args_of({}, w_out, p.M, p.O, p.F);
   u16* h = static_cast<u16*>(d->saved_h ? d->saved_h : ws.take(h_plane * NPH * 2));
   float* partial = static_cast<float*>(ws.take(partial_floats(out_args, splits_of<ELEM, NPH, NPL, true, true>(out_args)) * 4));
   if (!run) return ws.off;
@@ -687,7 +688,7 @@ int64_t forward(const cradle_gated_mlp_desc* d, const Plan& p, void* workspace, 
   const Operand hop{h, p.Fp, h_plane, 0};
   Finish finish;
   product_out<ELEM, NPH, NPL, true, true>(
-      args_of(hop, w_out, p.M, p.O, p.Fp),
+      args_of(hop, w_out, p.M, p.O, p.F),
       OutEpi{d->y, d->ld_y, p.dtype, d->b_out, d->residual, d->ld_residual, p.M, kNoGap, 0, p.O, vec_ok(d->y, d->ld_y, p.dtype)}, partial, finish, s);
   run_finish(finish, s);
   return ws.off;
