@@ -5,7 +5,7 @@
 // Numbers: X, S and B = b S + c S S are kept as two fp16 planes (hi + lo, 22 bits), three products per element pair with fp32
 // accumulation.  The iteration is normalised, |X_ij| <= |X|_2 <= max |p(s)|, so fp16's range is no obstacle: everything is held
 // times 2^12, which puts the lo plane of an entry of size 2^-6 (a 4096-wide matrix) well above fp16's subnormals and keeps
-// |X| < 16 (checked for the coefficients by the caller) below its largest number.  fp32 results at three products of a rate
+// |X|, |S| = |X|^2 and |B| below 15.9 (checked for the coefficients by the caller) below its largest number.  fp32 results at three products of a rate
 // 16 times the fp32 matrix instruction's.  fp16 tensors take the same path: one plane's error would show in their last bits.
 // bf16 tensors multiply with the hi plane alone in all but the last two steps (X itself, and a X, keep both): early on the
 // singular values are small and so is everything (b S + c S S) X adds, so its 11-bit error barely reaches the result -- in an

@@ -659,36 +659,56 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
-@functools.lru_cache(maxsize=64)
-def _ns_bound(coeffs, steps: int) -> float:
-    """Largest magnitude that s and b s^2 + c s^4 take over the iteration s <- a s + b s^3 + c s^5 from any s in [0, 1]."""
+# X, b S + c S S and S (whose eigenvalues are s^2) are held times 2^12 in fp16 planes, whose largest number is 65504: all below 15.9
+NS_LIMIT, NS_ENTER = 7.95, 3.98
+
+
+def _ns_range(coeffs, steps: int):
+    """Largest magnitudes over the iteration s <- a s + b s^3 + c s^5 from any s in [0, 1]: of s and b s^2 + c s^4 anywhere,
+    and of the s that enter a step."""
     a, b, c = (float(v) for v in coeffs)
     if not all(abs(v) < float("inf") for v in (a, b, c)):
-        return float("inf")
-    s, most = torch.linspace(0, 1, 4097, dtype=torch.float64, device="cpu"), 1.0
+        return float("inf"), float("inf")
+    s, most, entering = torch.linspace(0, 1, 4097, dtype=torch.float64, device="cpu"), 1.0, 1.0
     for _ in range(steps):
+        entering = max(entering, float(s.abs().max()))
         q = b * s * s + c * s ** 4
         s = a * s + q * s
         most = max(most, float(q.abs().max()), float(s.abs().max()))
         if not most < 1e6:
-            return float("inf")
+            return float("inf"), float("inf")
         s = torch.linspace(0, float(s.abs().max()), 4097, dtype=torch.float64, device="cpu")  # (every value between: a superset)
-    return most
+    return most, entering
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_bound(coeffs, steps: int) -> float:
+    """Largest magnitude that s and b s^2 + c s^4 take over the iteration s <- a s + b s^3 + c s^5 from any s in [0, 1]."""
+    return _ns_range(coeffs, steps)[0]
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_holds(coeffs, steps: int) -> bool:
+    """Whether everything the iteration holds stays in the planes' range."""
+    most, entering = _ns_range(coeffs, steps)
+    return most < NS_LIMIT and entering < NS_ENTER
 
 
 def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of each matrix of ``g`` (..., m, n), fp32 / bf16 / fp16: X = G / (|G|_F + eps), then
     ``steps`` times X <- a X + (b S + c S S) X with S = X X^T on the smaller side (``cradle_orthogonalize``); every singular value s
     goes through a s + b s^3 + c s^5.  fp32 accuracy inside, one rounding to g's type.  ``out`` may be ``g``.  Coefficients
-    whose iteration leaves (-8, 8) from a start in [0, 1] are refused (the products hold X times 2^12 in fp16 planes)."""
+    whose iteration from a start in [0, 1] reaches 7.95, or brings 3.98 (S: 15.9) into another step, are refused (the
+    products hold X, S and b S + c S S times 2^12 in fp16 planes)."""
     what = "orthogonalize"
     if not g.is_cuda or g.dtype not in FLOAT_TYPES or g.dim() < 2:
         raise hip.CradleHipError(f"{what}: expected (..., m, n) fp32 / bf16 / fp16 on the GPU, got {g.dtype} {tuple(g.shape)} on {g.device}")
     if not 1 <= int(steps) <= 64 or not 0 <= eps < float("inf"):
         raise hip.CradleHipError(f"{what}: steps={steps} (1..64), eps={eps}")
     coeffs = tuple(float(v) for v in coeffs)
-    if len(coeffs) != 3 or not _ns_bound(coeffs, int(steps)) < 8:
-        raise hip.CradleHipError(f"{what}: the iteration with coefficients {coeffs} does not stay within (-8, 8)")
+    if len(coeffs) != 3 or not _ns_holds(coeffs, int(steps)):
+        raise hip.CradleHipError(f"{what}: {steps} steps with coefficients {coeffs} do not stay below {NS_LIMIT}, and below {NS_ENTER} "
+                                 "between steps")
     m, n = g.shape[-2:]
     if out is None:
         out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
