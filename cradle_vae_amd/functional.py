@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -217,6 +218,14 @@ def onehot_linear(mask: torch.Tensor, W: torch.Tensor, b: torch.Tensor, t0: int 
 # A backward pass captured into a graph: let go of every eager graph over the same leaves before the capture (autograd runs a leaf's
 # accumulation on the stream its node was made on).
 # ---------------------------------------------------------------------------------------------
+def _differentiated(*tensors) -> bool:
+    """Whether a derivative of any of them is wanted: a gradient, or -- to be refused by autograd, these functions have no
+    forward-mode form -- a dual number's tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -239,7 +248,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last axis with its gradients (``ops.layer_norm``): fp32 / bf16 / fp16, parameters of x's type or
     fp32."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     return ops.layer_norm(x, weight, bias, eps)[0]
 
@@ -266,6 +275,6 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
               b_out: Optional[torch.Tensor] = None, act: str = "silu", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gated feed-forward block with its gradients: (act(g) * u) w_out^T + b_out (+ residual), [g | u] = x w_in^T + b_in
     (``ops.gated_mlp``).  Without anything to differentiate nothing is saved."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out, residual)):
+    if _differentiated(x, w_in, w_out, b_in, b_out, residual):
         return _GatedMLP.apply(x, w_in, w_out, b_in, b_out, residual, act)
     return ops.gated_mlp(x, w_in, w_out, b_in, b_out, act=act, residual=residual)
