@@ -61,6 +61,9 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
 // sum, in region order, of per-region sums S_i, each computed by the same two kernels below whoever computes it
 // -- the rank that owns region i after a reduce-scatter, or every rank over all regions after an all-reduce --
 // so that both ways of synchronising gradients give bit-identical clip coefficients.
+// The sums run in fp64 and travel as two fp32 numbers (hi + lo, 48 bits), so that another cut of the arena changes the norm
+// by 1e-14 and its fp32 value practically never: summed in fp32, two and four buckets gave norms one step apart, and four Adam
+// steps of a small model (whose clip is active) turned that into 2e-5 of a parameter.  The loads bound the pass either way.
 constexpr int kMaxRegions = 64;
 struct Regions {
   int64_t off[kMaxRegions];
@@ -69,29 +72,40 @@ struct Regions {
   int blocks;  // partial-sum workgroups per region
 };
 
-__global__ __launch_bounds__(256) void region_sumsq_kernel(const float* __restrict__ g, Regions r, float* __restrict__ part) {
-  __shared__ float red[4];
+__device__ __forceinline__ double block_sum_f64(double v, double* slot) {
+  for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
+  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (slot[0] + slot[1]) + (slot[2] + slot[3]);
+}
+
+__global__ __launch_bounds__(256) void region_sumsq_kernel(const float* __restrict__ g, Regions r, double* __restrict__ part) {
+  __shared__ double red[4];
   const int i = blockIdx.y;
   const float* src = g + r.off[i];
   const int64_t n = r.len[i], n4 = n >> 2;  // regions start 16-byte aligned (checked on the host)
   const float4* g4 = reinterpret_cast<const float4*>(src);
-  float acc = 0.f;
+  double acc = 0;
   for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n4; k += (int64_t)gridDim.x * 256) {
     const float4 v = g4[k];
-    acc += (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w);
+    acc += ((double)v.x * v.x + (double)v.y * v.y) + ((double)v.z * v.z + (double)v.w * v.w);
   }
   if (blockIdx.x == 0)
-    for (int64_t k = (n4 << 2) + threadIdx.x; k < n; k += 256) acc += src[k] * src[k];
-  acc = block_sum<256>(acc, red);
+    for (int64_t k = (n4 << 2) + threadIdx.x; k < n; k += 256) acc += (double)src[k] * src[k];
+  acc = block_sum_f64(acc, red);
   if (threadIdx.x == 0) part[(int64_t)i * gridDim.x + blockIdx.x] = acc;
 }
 
-__global__ __launch_bounds__(256) void region_finish_kernel(const float* __restrict__ part, int blocks, float* __restrict__ sums) {
-  __shared__ float red[4];
-  float acc = 0.f;
+// stride 1: the sums in fp32; 2: as hi, lo
+__global__ __launch_bounds__(256) void region_finish_kernel(const double* __restrict__ part, int blocks, int stride, float* __restrict__ sums) {
+  __shared__ double red[4];
+  double acc = 0;
   for (int k = threadIdx.x; k < blocks; k += 256) acc += part[(int64_t)blockIdx.x * blocks + k];
-  acc = block_sum<256>(acc, red);
-  if (threadIdx.x == 0) sums[blockIdx.x] = acc;
+  acc = block_sum_f64(acc, red);
+  if (threadIdx.x != 0) return;
+  const float hi = (float)acc;
+  sums[(int64_t)blockIdx.x * stride] = hi;
+  if (stride == 2) sums[(int64_t)blockIdx.x * 2 + 1] = (float)(acc - (double)hi);
 }
 
 __global__ __launch_bounds__(256) void adam_regions_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
@@ -99,9 +113,10 @@ __global__ __launch_bounds__(256) void adam_regions_kernel(float* __restrict__ p
                                                            float eps, float wd, float bc1, float sqrt_bc2, float max_norm,
                                                            float grad_scale, const float* __restrict__ all_sums, int n_sums,
                                                            float* __restrict__ norm_out, const int* __restrict__ skip_flags) {
-  float tot = 0.f;
-  for (int k = 0; k < n_sums; ++k) tot += all_sums[k];  // fixed order, the same on every rank
-  const float norm = sqrtf(tot) * fabsf(grad_scale);
+  double sum = 0;
+  for (int k = 0; k < n_sums; ++k) sum += (double)all_sums[k];  // fixed order, the same on every rank
+  const float tot = (float)sum;
+  const float norm = (float)sqrt(sum) * fabsf(grad_scale);
   const bool first = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
   // A rank whose step rejected its input puts a NaN into its gradients before they are summed
   // (cradle_grad_poison_if_flagged): the sum of squares every rank sees is then not finite and ALL ranks skip the
@@ -177,20 +192,31 @@ int cradle_adam_step(float* params, const float* grads, float* exp_avg, float* e
 
 int64_t cradle_adam_workspace_floats(void) { return cradle::kNormBlocks + 1; }
 
+static int region_sumsq(const char* what, const float* grads, const int64_t* region_off, const int64_t* region_len, int n_regions,
+                        int n_total, int stride, float* region_sums, float* ws, hipStream_t stream) {
+  using namespace cradle;
+  CRADLE_CHECK_ARG(grads && region_sums && ws && (uintptr_t)grads % 16 == 0 && (uintptr_t)ws % 8 == 0, "%s: bad arguments", what);
+  Regions r;
+  const int rc = fill_regions(r, region_off, region_len, n_regions, n_total, what);
+  if (rc) return rc;
+  double* part = reinterpret_cast<double*>(ws);
+  hipLaunchKernelGGL(region_sumsq_kernel, dim3(r.blocks, r.n), dim3(256), 0, stream, grads, r, part);
+  hipLaunchKernelGGL(region_finish_kernel, dim3(r.n), dim3(256), 0, stream, part, r.blocks, stride, region_sums);
+  CRADLE_CHECK_LAUNCH(what);
+  return CRADLE_OK;
+}
+
 // region_sums[i] = sum of squares of grads over region i (offsets / lengths in floats, host arrays), i < n_regions;
 // n_total = number of regions the whole arena is cut into (fixes the summation order, see above).
 // ws: cradle_adam_regions_workspace_floats() floats.
 int cradle_grad_region_sumsq(const float* grads, const int64_t* region_off, const int64_t* region_len, int n_regions,
                              int n_total, float* region_sums, float* ws, hipStream_t stream) {
-  using namespace cradle;
-  CRADLE_CHECK_ARG(grads && region_sums && ws && (uintptr_t)grads % 16 == 0, "grad_region_sumsq: bad arguments");
-  Regions r;
-  const int rc = fill_regions(r, region_off, region_len, n_regions, n_total, "grad_region_sumsq");
-  if (rc) return rc;
-  hipLaunchKernelGGL(region_sumsq_kernel, dim3(r.blocks, r.n), dim3(256), 0, stream, grads, r, ws);
-  hipLaunchKernelGGL(region_finish_kernel, dim3(r.n), dim3(256), 0, stream, ws, r.blocks, region_sums);
-  CRADLE_CHECK_LAUNCH("grad_region_sumsq");
-  return CRADLE_OK;
+  return region_sumsq("grad_region_sumsq", grads, region_off, region_len, n_regions, n_total, 1, region_sums, ws, stream);
+}
+// The same with two floats per region, whose sum is the region's to 48 bits.
+int cradle_grad_region_sumsq_pairs(const float* grads, const int64_t* region_off, const int64_t* region_len, int n_regions,
+                                   int n_total, float* region_sums, float* ws, hipStream_t stream) {
+  return region_sumsq("grad_region_sumsq_pairs", grads, region_off, region_len, n_regions, n_total, 2, region_sums, ws, stream);
 }
 
 int64_t cradle_adam_regions_workspace_floats(void) { return (int64_t)cradle::kMaxRegions * 512; }
@@ -207,7 +233,7 @@ int cradle_grad_poison_if_flagged(float* element, const int* flags, hipStream_t 
 }
 
 // cradle_adam_step on the listed regions only, with the gradient's squared norm given as all_sums (device,
-// n_sums region sums of the whole arena, added in order).  norm_out (device float[2], may be NULL): [0] receives
+// n_sums numbers whose sum it is: a float or a pair of them per region of the whole arena, added in order).  norm_out (device float[2], may be NULL): [0] receives
 // |g'|, [1] is incremented whenever the update is skipped (skip_flags set, or the squared norm not finite).
 int cradle_adam_step_regions(float* params, const float* grads, float* exp_avg, float* exp_avg_sq,
                              const int64_t* region_off, const int64_t* region_len, int n_regions, const float* all_sums,
@@ -216,7 +242,9 @@ int cradle_adam_step_regions(float* params, const float* grads, float* exp_avg, 
   using namespace cradle;
   CRADLE_CHECK_ARG(params && grads && exp_avg && exp_avg_sq && all_sums && step >= 1, "adam_step_regions: bad arguments");
   Regions r;
-  const int rc = fill_regions(r, region_off, region_len, n_regions, n_sums, "adam_step_regions");
+  CRADLE_CHECK_ARG(n_sums >= n_regions && n_sums <= 2 * kMaxRegions, "adam_step_regions: %d sums for %d regions (at most %d)", n_sums,
+                   n_regions, 2 * kMaxRegions);
+  const int rc = fill_regions(r, region_off, region_len, n_regions, n_regions, "adam_step_regions");
   if (rc) return rc;
   int64_t longest = 0;
   for (int i = 0; i < r.n; ++i) longest = longest > r.len[i] ? longest : r.len[i];

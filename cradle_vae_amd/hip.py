@@ -78,6 +78,8 @@ PROTOTYPES = {
     "cradle_adam_workspace_floats": (i64, []),
     "cradle_grad_region_sumsq": (i32, [c_float_p, ctypes.POINTER(i64), ctypes.POINTER(i64), i32, i32, c_float_p, c_float_p,
                                        c_stream]),
+    "cradle_grad_region_sumsq_pairs": (i32, [c_float_p, ctypes.POINTER(i64), ctypes.POINTER(i64), i32, i32, c_float_p, c_float_p,
+                                             c_stream]),
     "cradle_adam_regions_workspace_floats": (i64, []),
     "cradle_adam_step_regions": (
         i32,
@@ -125,7 +127,7 @@ PROTOTYPES = {
 }
 
 MAX_LAYERS = 8
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 
 class MlpPtrs(ctypes.Structure):

@@ -120,7 +120,7 @@ class TrainStep:
         self._my_regions = (arr([o for o, _ in mine]), arr([n for _, n in mine]), len(mine))
         lib = hip.load()
         self.region_ws = torch.zeros(lib.cradle_adam_regions_workspace_floats(), device=self.device)
-        self.region_sums = torch.zeros(len(flat), device=self.device)
+        self.region_sums = torch.zeros(2 * len(flat), device=self.device)  # (hi, lo) of every region's sum
         self.norm_out = torch.zeros(2, device=self.device)  # [|g|, updates skipped on every rank since the last look]
         self.fused.defer_flag_check = True  # ranks raise together (check_flags), never one alone inside FusedElboStep.run
 
@@ -140,8 +140,8 @@ class TrainStep:
         from . import hip
 
         off, ln, n = regions
-        hip.check(hip.load().cradle_grad_region_sumsq(a.grad.data_ptr(), off, ln, n, self._all_regions[2], out.data_ptr(),
-                                                      self.region_ws.data_ptr(), hip.stream()), "cradle_grad_region_sumsq")
+        hip.check(hip.load().cradle_grad_region_sumsq_pairs(a.grad.data_ptr(), off, ln, n, self._all_regions[2], out.data_ptr(),
+                                                            self.region_ws.data_ptr(), hip.stream()), "cradle_grad_region_sumsq_pairs")
 
     def draw_noise(self, P, N):
         g = self.lm.guide
@@ -216,7 +216,7 @@ class TrainStep:
                 cur.wait_stream(self.comm_stream)
         # |g|^2 = in-order sum of the region sums (bucket x rank), whoever computes them
         if shard:
-            mine = self.region_sums[:self._my_regions[2]]
+            mine = self.region_sums[:2 * self._my_regions[2]]
             self._region_sumsq(a, self._my_regions, mine)
             all_sums = parallel.all_gather_small(mine, gw)
             self._adam_regions(a, self._my_regions, all_sums)

@@ -317,9 +317,11 @@ int64_t cradle_adam_workspace_floats(void);
  * computed the same way by whoever computes it, so that reduce-scatter + sharded update + all-gather and all-reduce +
  * full update give bit-identical parameters.
  *   cradle_grad_region_sumsq : region_sums[i] = sum_{region i} grads^2 for the n_regions listed regions (ws:
- *                              cradle_adam_regions_workspace_floats() floats)
- *   cradle_adam_step_regions : clip + Adam on the listed regions only; all_sums (device, n_sums = n_total) = the region
- *                              sums of the whole arena (all-gathered over ranks); norm_out (device float[2], may be
+ *                              cradle_adam_regions_workspace_floats() floats, 8-byte aligned)
+ *   cradle_grad_region_sumsq_pairs : the same as region_sums[2 i] + region_sums[2 i + 1], 48 bits of an fp64 sum, so that the
+ *                              norm does not depend on how the arena is cut
+ *   cradle_adam_step_regions : clip + Adam on the listed regions only; all_sums (device, n_sums = n_total, or 2 n_total of
+ *                              pairs) = the region sums of the whole arena (all-gathered over ranks); norm_out (device float[2], may be
  *                              NULL): [0] receives |g'|, [1] is incremented whenever the update is skipped -- skip_flags
  *                              non-zero, or the squared norm not finite
  *   cradle_grad_poison_if_flagged : writes NaN into *element (a float of the gradient arena that is summed over ranks
@@ -328,6 +330,8 @@ int64_t cradle_adam_workspace_floats(void);
  *                              Lightning DDP (train_norman.py:89-97) every rank applies the same update or none */
 int cradle_grad_region_sumsq(const float* grads, const int64_t* region_off, const int64_t* region_len, int n_regions,
                              int n_total, float* region_sums, float* ws, cradle_stream_t stream);
+int cradle_grad_region_sumsq_pairs(const float* grads, const int64_t* region_off, const int64_t* region_len, int n_regions,
+                                   int n_total, float* region_sums, float* ws, cradle_stream_t stream);
 int64_t cradle_adam_regions_workspace_floats(void);
 int cradle_adam_step_regions(float* params, const float* grads, float* exp_avg, float* exp_avg_sq,
                              const int64_t* region_off, const int64_t* region_len, int n_regions, const float* all_sums,
