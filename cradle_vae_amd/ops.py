@@ -451,8 +451,8 @@ def _rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
 
 
 def _ld(t: torch.Tensor) -> int:
-    ld, (rows, cols) = t.stride(0), t.shape
-    return ld if rows > 1 or ld > cols else cols
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols  # (a single row's stride is its parent's and is never used)
 
 
 def _same_place(what: str, ref: torch.Tensor, **others) -> None:
@@ -567,6 +567,12 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
+def _tile_rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``_rows_of`` for an operand of tile products, whose leading dimension has to stay below 2^22: copied above."""
+    r = _rows_of(t, what)
+    return r if _ld(r) < 1 << 22 else r.contiguous()
+
+
 def _gated_desc(what, x, w_in, w_out, act):
     if act not in ACTIVATIONS:
         raise hip.CradleHipError(f"{what}: act={act!r}, expected one of {sorted(ACTIVATIONS)}")
@@ -577,7 +583,9 @@ def _gated_desc(what, x, w_in, w_out, act):
     if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
         raise hip.CradleHipError(f"{what}: x is {x.dtype}, w_in {w_in.dtype}, w_out {w_out.dtype}")
     _same_place(what, x, w_in=w_in, w_out=w_out)
-    x2, wi, wo = _rows_of(x, what), _rows_of(w_in, what), _rows_of(w_out, what)
+    x2, wi, wo = _tile_rows(x, what), _tile_rows(w_in, what), _tile_rows(w_out, what)
+    if (wo.shape[1] + 320) * ((_ld(wi) + 63) // 64 * 64) >= 1 << 30:
+        wi = wi.contiguous()
     d = hip.GatedMlpDesc()
     d.rows, d.width, d.hidden, d.out_width = x2.shape[0], x2.shape[1], wo.shape[1], wo.shape[0]
     d.dtype, d.act = FLOAT_TYPES[x.dtype], ACTIVATIONS[act]
@@ -646,7 +654,7 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
     dw_in, dw_out = (new((2 * F, K)) if need[1] else None), (new((O, F)) if need[2] else None)
     db_in, db_out = (new((2 * F,)), new((O,))) if bias else (None, None)
     if M:
-        dy2 = _rows_of(dy, what)
+        dy2 = _tile_rows(dy, what)
         d.dy, d.ld_dy, d.saved_gu, d.saved_h = dy2.data_ptr(), _ld(dy2), saved[0].data_ptr(), saved[1].data_ptr()
         d.dx, d.ld_dx, d.dw_in, d.dw_out, d.db_in, d.db_out = (_pointer(dx), K, _pointer(dw_in), _pointer(dw_out), _pointer(db_in),
                                                                _pointer(db_out))

@@ -32,3 +32,28 @@ def test_weights_inside_wider_buffers_with_a_padded_hidden_axis(dtype):
     ref.close(y, want["y"][0], want["y"][1], "y")
     for name, got in zip(NAMES, ops.gated_mlp_bwd(_in_nan(dy, 128), gx, gi, go, saved, bias=True)):
         ref.close(got, want[name][0], want[name][1], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 2, 20])
+def test_rows_far_apart(rows, dtype):
+    # row strides of 2^22 + 8 numbers (one row: its parent's, which nobody uses); weights that span 2^30 numbers
+    x, w_in, w_out, b_in, b_out, dy = _inputs(rows, 40, 24, 16, dtype)
+    want, _ = ref.gated_mlp(x, w_in, w_out, b_in, b_out, dy, "silu")
+    far = (1 << 22) + 8
+
+    def apart(t, ld):
+        buf = torch.empty(t.shape[0] * ld, dtype=dtype, device="cuda")
+        view = buf.as_strided(t.shape, (ld, 1))
+        view.copy_(t)
+        return view
+
+    gx, gd, gi, go = apart(x, far), apart(dy, far), apart(w_in, 1 << 21 if dtype == torch.bfloat16 else 48), w_out.cuda()
+    b = b_in.cuda(), b_out.cuda()
+    ref.close(ops.gated_mlp(gx, gi, go, *b), want["y"][0], want["y"][1], "y (inference)")
+    y, saved = ops.gated_mlp(gx, gi, go, *b, save=True)
+    ref.close(y, want["y"][0], want["y"][1], "y")
+    for name, got in zip(NAMES, ops.gated_mlp_bwd(gd, gx, gi, go, saved, bias=True)):
+        ref.close(got, want[name][0], want[name][1], name)
+    mean, rstd = ops.layer_norm(gx)[1:]
+    assert torch.equal(ops.layer_norm_bwd(gx, gx, None, mean, rstd)[0], ops.layer_norm_bwd(x.cuda(), x.cuda(), None, mean, rstd)[0])
