@@ -25,7 +25,9 @@ class TrainStep:
         self.clip = gradient_clip_norm
         self.params = [p for p in loss_module.parameters() if p.requires_grad]
         self.optimizer_name = optimizer
-        self.optimizer = make_optimizer(optimizer, loss_module, lr, weight_decay)
+        # (only what trains: a frozen parameter with an old gradient would move by its weight decay)
+        self.optimizer = (torch.optim.Adam(self.params, lr=lr, weight_decay=weight_decay) if optimizer == "adam"
+                          else make_optimizer(optimizer, loss_module, lr, weight_decay))
         self.device = self.params[0].device
         # plated draws (mask, E, qc_E) must agree across ranks, local draws (z_basal) must not:
         # two generators, the first seeded identically everywhere
