@@ -122,11 +122,16 @@ class GaussianLikelihoodResidualMLP(nn.Module):
         mean, var = self.mean_var(x)
         return torch.distributions.Normal(mean, var.sqrt(), validate_args=False)
 
-    def forward_from_hidden(self, h: torch.Tensor) -> torch.distributions.Normal:
+    def forward_from_hidden(self, h: torch.Tensor, first_layer_done: bool = True) -> torch.distributions.Normal:
         """The rest of forward() given the first trunk layer's output h (..., H) (the caller evaluated that layer
-        in a cheaper form: guide._embedding_dist)."""
+        in a cheaper form: guide._embedding_dist); with ``first_layer_done=False`` that layer is applied to h like a
+        further residual one."""
         shape = h.shape
-        z = self.mlp.tail(h.reshape(-1, shape[-1]))
+        z = h.reshape(-1, shape[-1])
+        if not first_layer_done:
+            lin = self.mlp.linears()[0]
+            z = F_hip.linear(z, lin.weight, lin.bias, act=True, residual=z)
+        z = self.mlp.tail(z)
         mean = F_hip.linear(z, self.mean_encoder.weight, self.mean_encoder.bias)
         var = torch.exp(F_hip.linear(z, self.log_var_encoder.weight, self.log_var_encoder.bias)) + self.var_eps
         mean = nan_to_num_ref(mean.reshape(*shape[:-1], -1))
