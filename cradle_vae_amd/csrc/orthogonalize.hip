@@ -97,11 +97,11 @@ __global__ __launch_bounds__(256) void pack_kernel(const Tensor g, const double*
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   s = (red[0] + red[1]) + (red[2] + red[3]);
-  const float scale = kScale / ((float)sqrt(s) + eps);
+  const double scale = kScale / (sqrt(s) + (double)eps);  // (in fp64: the norm or its reciprocal can lie beyond fp32)
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int r = k * 4 + threadIdx.x / 64;
-    tile[r][c] = g0 + r < g.rows && g1 + c < g.cols ? v[k] * scale : 0.f;
+    tile[r][c] = g0 + r < g.rows && g1 + c < g.cols ? (float)(v[k] * scale) : 0.f;
   }
   __syncthreads();
   u16* out = x + (int64_t)blockIdx.z * batch;
@@ -401,12 +401,15 @@ __global__ __launch_bounds__(kSmallThreads, 1) void small_kernel(const Tensor g,
   s = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) s += red[w];
-  const float scale = kScale / ((float)sqrt(s) + eps);
+  const double scale = kScale / (sqrt(s) + (double)eps);  // (in fp64: the norm or its reciprocal can lie beyond fp32)
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
     const int t = i * kSmallThreads + threadIdx.x;
     const int r = flip ? t % MP : t / (NP / 4), c0 = (flip ? t / MP : t % (NP / 4)) * 4;
-    store_planes<F16, 2>(small_at<NP>(X, r, c0), (int64_t)XP * 8, x[i] * scale);
+    f32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = (float)(x[i][e] * scale);
+    store_planes<F16, 2>(small_at<NP>(X, r, c0), (int64_t)XP * 8, w);
   }
   __syncthreads();
 

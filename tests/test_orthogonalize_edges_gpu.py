@@ -21,3 +21,20 @@ def test_coefficients_just_inside_the_range(m, n, coeffs, steps):
     # 16.8 - 23.7 = -7.0: B X is off by 2 * 23.7, a X by 16.8, and the step before by 3.9 times the slope 13.9, all 2^-21 and
     # beside 7.0: 17 of them; twice that
     assert float((got - want).norm() / want.norm()) <= 34 * 2.0 ** -21
+
+
+@pytest.mark.parametrize("m,n", [(48, 72), (200, 144)])
+def test_norms_beyond_fp32(m, n):
+    g = _matrix(1, m, n, torch.float32, scale=1.0)
+    want = ref.orthogonalize(g, 5, ops.NS_COEFFS, eps=0.0)
+    # |g| near 2^130, whose fp32 value is infinite, and near 2^-117, whose reciprocal times 2^12 is
+    for scale in (2.0 ** 123, 2.0 ** -126):
+        x = g * scale
+        assert bool(torch.isfinite(x).all())
+        got = ops.orthogonalize(x.cuda(), eps=0.0).double().cpu()
+        plain = ref.orthogonalize(g, 5, ops.NS_COEFFS, eps=0.0, dtype=torch.float32).double()
+        # as at any scale four times fp32's own error and its rounding; numbers below 2^-126 have lost up to 2^-150 each, beside
+        # the norm 2^-25 for sqrt(m n) of them, amplified by at most 3.44 a step
+        own = float((plain - want).norm() / want.norm())
+        assert float((got - want).norm() / want.norm()) <= 4 * own + 8 * ref.U + (2.0 ** -25 * 3.45 ** 5 if scale < 1 else 0.0)
+    assert float(ops.orthogonalize(torch.zeros(1, m, n, device="cuda")).abs().max()) == 0
