@@ -29,19 +29,26 @@ enum Act { SILU = 0, GELU = 1 };
 
 // act(g) and act'(g), in a handful of instructions: an epilogue has one or two waves per SIMD and nothing to hide long sequences
 // behind (with the library's expf, erfcf and divisions the first backward product of 1537 x 1000 x 2731 takes 45 us).
-// silu: g s, s = 1 / (1 + exp(-g)) on the hardware's exp2 and reciprocal, a few 2^-24 relative.
-// gelu: g Phi(g), Phi(-|g|) = (a1 t + ... + a5 t^5) exp(-g^2 / 2) / 2, t = 1 / (1 + 0.3275911 |g| / sqrt(2)): the rational
-// approximation 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions, off by at most 0.75e-7.
+// silu: g s, s = 1 / (1 + exp(-g)) on the hardware's exp2 and reciprocal: relative to s off by (1 - s) (1.5 |g| + 3) + 2 times
+// 2^-24, the exponent's argument being rounded (|g| s (1 - s) is at most 0.23, so that is no more than act's own rounding).
+// gelu: g Phi(g).  FINE (fp32 tensors): Phi(g) = erfc(-g / sqrt(2)) / 2 by the library's erfcf, accurate relative to Phi down its
+// tail.  Otherwise (16-bit tensors, whose half step is 2^-12 and more) Phi(-|g|) = (a1 t + ... + a5 t^5) exp(-g^2 / 2) / 2, t =
+// 1 / (1 + 0.3275911 |g| / sqrt(2)): the rational approximation 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical
+// Functions, off by at most 0.75e-7, and 2.3e-7 (2^-22) as evaluated in fp32.
 // Limits: a gate of 0 with its argument infinite is 0.
 __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
 }
-// Phi(g); e = exp(-g^2 / 2)
+__device__ __forceinline__ float gauss(float g) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g); }  // exp(-g^2 / 2)
+// Phi(g); e = gauss(g)
+template <bool FINE>
 __device__ __forceinline__ float normal_cdf(float g, float e) {
+  if constexpr (FINE) return 0.5f * erfcf(-0.70710678118654752f * g);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.23164188f, fabsf(g), 1.f));
   const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f) * e;
   return g < 0.f ? q : 1.f - q;
 }
+template <bool FINE>
 __device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
   if (act == SILU) {
     const float s = sigmoid(g);
@@ -49,14 +56,15 @@ __device__ __forceinline__ void act_both(int act, float g, float& a, float& da) 
     da = s == 0.f ? 0.f : s * fmaf(g, 1.f - s, 1.f);
     if (g == INFINITY) da = 1.f;
   } else {
-    const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
-    const float cdf = normal_cdf(g, e);
+    const float e = gauss(g);
+    const float cdf = normal_cdf<FINE>(g, e);
     a = cdf == 0.f ? 0.f : g * cdf;
     da = e == 0.f ? cdf : fmaf(g * 0.39894228040143268f, e, cdf);
   }
 }
+template <bool FINE>
 __device__ __forceinline__ float act_only(int act, float g) {
-  const float s = act == SILU ? sigmoid(g) : normal_cdf(g, __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g));
+  const float s = act == SILU ? sigmoid(g) : normal_cdf<FINE>(g, gauss(g));
   return s == 0.f ? 0.f : g * s;
 }
 
@@ -168,7 +176,7 @@ struct GateEpi {
       const f32x4 g = *p + b.v, u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + T::WN / 2) + b.w;
       f32x4 h4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h4[e] = n + e < hidden ? act_only(act, g[e]) * u[e] : 0.f;
+      for (int e = 0; e < 4; ++e) h4[e] = n + e < hidden ? act_only<NPH == 3>(act, g[e]) * u[e] : 0.f;
       store_planes<ELEM, NPH>(h + (int64_t)m * hidden_p + n, h_plane, h4);
       if (gu) {
         float* o = gu + (int64_t)m * 2 * hidden_p + n;
@@ -208,7 +216,7 @@ struct GateBwdEpi {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float av, dav;
-        act_both(act, g[e], av, dav);
+        act_both<NPD == 3>(act, g[e], av, dav);
         const bool in = n + e < hidden;
         dg[e] = in ? dh[e] * u[e] * dav : 0.f;
         du[e] = in ? dh[e] * av : 0.f;

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const void* __restrict__ 
         s0 += load_as(bias, n, DT);
         s1 += load_as(bias, (int64_t)N + n, DT);
       }
-      if (lane == 0) h[(int64_t)r * N + n] = act_only(act, s0) * s1;
+      if (lane == 0) h[(int64_t)r * N + n] = act_only<DT == CRADLE_F32>(act, s0) * s1;
     } else if (lane == 0) {
       if (bias) s0 += load_as(bias, n, DT);
       if (res) s0 += load_as(res, (int64_t)r * ld_res + n, DT);

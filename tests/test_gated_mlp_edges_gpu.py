@@ -1,5 +1,7 @@
 """The gated feed-forward block where its operands are staged in unusual ways: views inside wider buffers at sizes that
 pad the hidden axis, long row strides, and the fp32 products' planes."""
+import math
+
 import pytest
 import torch
 
@@ -57,3 +59,38 @@ def test_rows_far_apart(rows, dtype):
         ref.close(got, want[name][0], want[name][1], name)
     mean, rstd = ops.layer_norm(gx)[1:]
     assert torch.equal(ops.layer_norm_bwd(gx, gx, None, mean, rstd)[0], ops.layer_norm_bwd(x.cuda(), x.cuda(), None, mean, rstd)[0])
+
+
+def _gate_alone(act, g):
+    """act(g) and act'(g) as the block's output and input gradient in fp32: one hidden unit whose up projection is 1, so that
+    nothing else is rounded (its one product is by 1)."""
+    x = g.reshape(-1, 1).cuda()
+    w_in, w_out, b_in = torch.tensor([[1.0], [0.0]]).cuda(), torch.ones(1, 1).cuda(), torch.tensor([0.0, 1.0]).cuda()
+    y, saved = ops.gated_mlp(x, w_in, w_out, b_in, None, act=act, save=True)
+    dx = ops.gated_mlp_bwd(torch.ones_like(y), x, w_in, w_out, saved, act=act)[0]
+    few = torch.cat([ops.gated_mlp(part, w_in, w_out, b_in, None, act=act) for part in x[:400].split(8)])
+    return (t.double().cpu().reshape(-1) for t in (y, dx, few))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_the_gate_in_fp32(act):
+    g = torch.cat([8 * torch.rand(200, generator=torch.Generator().manual_seed(0)) - 8, torch.linspace(-8, 8, 3801)]).float()
+    y, dx, few = _gate_alone(act, g)
+    d, U = g.double(), ref.U
+    if act == "silu":
+        # the exponent's argument: two roundings of up to 1.45 |g|, the hardware's exp2 and reciprocal one step each
+        s = torch.sigmoid(d)
+        want, dwant = d * s, s * (1 + d * (1 - s))
+        e_s = s * ((1 - s) * (1.5 * d.abs() + 3) + 3) * U
+        e_d = e_s * (1 + d.abs() * (1 - s)) + s * d.abs() * (e_s + U) + 4 * U * s * (1 + d.abs() * (1 - s))
+    else:
+        # erfc within four steps, its argument rounded twice: a relative error of its argument's square
+        s = 0.5 * torch.erfc(-d / math.sqrt(2))
+        pdf = torch.exp(-0.5 * d * d) / math.sqrt(2 * math.pi)
+        want, dwant = d * s, s + d * pdf
+        e_s = s * 8 * U + 1.5 * d.abs() * pdf * U
+        e_d = e_s + d.abs() * pdf * (2 * d * d + 8) * U + 2 * U * (s + d.abs() * pdf)
+    bound = d.abs() * e_s + 2 * U * want.abs()
+    assert bool(((y - want).abs() <= bound).all()), float(((y - want).abs() / bound.clamp_min(1e-300)).max())
+    assert bool(((few - want[:400]).abs() <= bound[:400]).all())
+    assert bool(((dx - dwant).abs() <= e_d + 2 * U * dwant.abs()).all()), float(((dx - dwant).abs() / (e_d + 2 * U * dwant.abs())).max())
