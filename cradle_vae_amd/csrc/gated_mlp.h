@@ -9,6 +9,8 @@
 // 2.6x the rate of the fp32 matrix instruction).  Sums, pre-activations and biases are fp32.  h and [dg | du] are inputs of a
 // matrix product and so are rounded once to the operand's type, an error of the size of the result's own last rounding; small
 // blocks, whose few numbers would not average it out and which are bound by latency, keep them in two planes instead.
+// In fp16 they have its range as well, with either number of planes: an h beyond 65504 is infinite, a [dg | du] below 2^-24 zero.
+// (bf16 planes beside fp16 tensors would keep fp32's range, at three products instead of one for four of the six.)
 // The saved pre-activations stay fp32 (rounded to bf16 they would put two more roundings into every gradient).
 // A handful of rows (inference of single cells) take kernels that read the weights once, coalesced, with fp32 arithmetic.
 //

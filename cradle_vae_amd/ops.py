@@ -607,7 +607,12 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     """Gated feed-forward block: [g | u] = x w_in^T + b_in; y = (act(g) * u) w_out^T + b_out (+ residual).  ``w_in``
     (2 hidden, width) holds the gate's rows, then the up projection's; ``act`` "silu" or "gelu" (erf); all tensors of one type, fp32 /
     bf16 / fp16 (``cradle_gated_mlp_fwd``).  ``save``: -> (y, saved), what ``gated_mlp_bwd`` reads (the pre-activations in
-    fp32 and h); a few rows without ``save`` take the form for single cells, which reads the weights once."""
+    fp32 and h); a few rows without ``save`` take the form for single cells, which reads the weights once.
+
+    16-bit tensors: h and the gradients of g and u are inputs of matrix products and are rounded to the tensors' type on the way, to
+    twice its bits while rows * hidden * (width + out) < 2^28 (a larger batch is rounded more); the form for a few rows keeps
+    h in fp32.  They have the type's range too: in fp16 an h beyond 65504 is infinite and a gradient of g or u below 6e-8 is
+    zero, as in any fp16 network (scale the loss), also where y or the weights' gradients would be representable."""
     what = "gated_mlp"
     d, keep = _gated_desc(what, x, w_in, w_out, act)
     M, O, F = d.rows, d.out_width, d.hidden
@@ -638,7 +643,8 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
 def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, saved, *, act: str = "silu",
                   bias: bool = False, need=(True, True, True)):
     """-> (dx, dw_in, dw_out, db_in, db_out) of ``gated_mlp``; ``need`` says which of the first three are wanted (None in the
-    place of the others), ``bias`` whether the biases' gradients are.  The residual's gradient is dy itself."""
+    place of the others), ``bias`` whether the biases' gradients are.  The residual's gradient is dy itself.  The 16-bit types'
+    roundings and fp16's range: ``gated_mlp``."""
     what = "gated_mlp_bwd"
     d, keep = _gated_desc(what, x, w_in, w_out, act)
     M, K, O, F = d.rows, d.width, d.out_width, d.hidden

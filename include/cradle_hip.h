@@ -447,7 +447,8 @@ int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
  * cradle_gated_mlp_bwd: from dy (rows, out_width) and the saved buffers, dx (rows, width; NULL = not needed), dw_in, dw_out
  * (contiguous, NULL = not needed), db_in, db_out (NULL = not needed).  The residual's gradient is dy.
  * h and [dg | du] are rounded to the tensors' type where they enter a matrix product (fp32: to 24 bits; 16-bit types of small
- * blocks, rows * hidden * (width + out_width) < 2^28: to twice their bits).  fp32 inputs of
+ * blocks, rows * hidden * (width + out_width) < 2^28: to twice their bits, in the type's range all the same: in fp16 an h beyond
+ * 65504 becomes infinite and a dg or du below 6e-8 zero; a few rows at inference keep h in fp32).  fp32 inputs of
  * magnitude above 3.39e38 count as infinite.  workspace: cradle_gated_mlp_workspace_bytes(desc, backward) bytes, 16-byte aligned;
  * only the sizes, types, pointers' alignment and which pointers are NULL are read for it.
  * (hidden + 320) * ld_w_in (rounded up to 64) < 2^30, widths <= 2^20, leading dimensions < 2^22.  No output may overlap an input or
