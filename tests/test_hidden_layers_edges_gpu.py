@@ -4,7 +4,10 @@ import torch
 from torch.autograd import forward_ad
 
 from cradle_vae_amd import functional as F_hip
+from cradle_vae_amd import ops
 from cradle_vae_amd.mlp import GaussianLikelihoodResidualMLP
+from cradle_vae_amd.optim import Muon
+from tests import operator_reference as ref
 from tests.test_hidden_layers_gpu import DEV, _params
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +38,26 @@ def test_the_rest_of_a_head_from_its_first_layers_output(block):
     got = m.forward_from_hidden(h, first_layer_done=False)
     again = m.forward_from_hidden(F_hip.linear(h, lin.weight, lin.bias, act=True, residual=h))
     assert torch.equal(got.mean, again.mean) and torch.equal(got.stddev, again.stddev)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_hidden_matrices_of_every_type(dtype):
+    gen = torch.Generator().manual_seed(0)
+    ps = [torch.nn.Parameter((torch.randn(s, generator=gen) * 0.1).to(DEV, dtype)) for s in ((32, 48), (32, 48), (150, 130))]
+    opt = Muon(ps, lr=0.02, momentum=0.9, weight_decay=0.01)
+    want, buf = [p.detach().double().cpu() for p in ps], [torch.zeros(p.shape).double() for p in ps]
+    for _ in range(3):
+        for i, p in enumerate(ps):
+            p.grad = torch.randn(p.shape, generator=gen).to(DEV, dtype)
+            g = p.grad.double().cpu()
+            buf[i] = 0.9 * buf[i] + g
+            want[i] = want[i] * (1 - 0.02 * 0.01) - 0.02 * 0.2 * max(p.shape) ** 0.5 * ref.orthogonalize(g + 0.9 * buf[i], 5, ops.NS_COEFFS)
+        opt.step()
+    for i, p in enumerate(ps):
+        st = opt.state[p]["momentum"]
+        # three roundings of sums of two terms; per step an update of rms 0.2 off by at most 2e-5 of its norm, and one
+        # rounding of the parameter
+        assert st.dtype == torch.float32 and float((st.double().cpu() - buf[i]).norm()) <= 6 * ref.U * float(buf[i].norm()) * 2
+        off = 3 * 2e-5 * 0.02 * 0.2 * p.numel() ** 0.5 * 2 + 8 * ref.U * float(want[i].norm())
+        off += 3 * ref.HALF[dtype] * float(want[i].norm()) * 1.1
+        assert p.dtype == dtype and float((p.detach().double().cpu() - want[i]).norm()) <= off
