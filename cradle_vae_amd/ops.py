@@ -733,9 +733,11 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float 
     g3 = g if g.dim() == 3 else g.unsqueeze(0) if g.dim() == 2 else g.reshape(-1, m, n)
     if (n > 1 and g3.stride(2) != 1) or (m > 1 and g3.stride(1) < n) or g3.stride(0) < 0:
         g3 = g3.contiguous()
-    if out.untyped_storage().data_ptr() == g3.untyped_storage().data_ptr() and (out.data_ptr() != g3.data_ptr() or not g3.is_contiguous()):
-        g3 = g3.clone(memory_format=torch.contiguous_format)  # (a workgroup's result could overwrite another's matrix before it is read)
     B = g3.shape[0]
+    here, there = g3.data_ptr(), out.data_ptr()
+    end = here + ((B - 1) * g3.stride(0) + (m - 1) * g3.stride(1) + n) * g3.element_size()
+    if here < there + out.numel() * out.element_size() and there < end and (here != there or not g3.is_contiguous()):
+        g3 = g3.clone(memory_format=torch.contiguous_format)  # (a workgroup's result could overwrite another's matrix before it is read)
     ld = g3.stride(1) if m > 1 else max(g3.stride(1), n)
     lib = hip.load()
     need = lib.cradle_orthogonalize_workspace_bytes(B, m, n)

@@ -38,3 +38,17 @@ def test_norms_beyond_fp32(m, n):
         own = float((plain - want).norm() / want.norm())
         assert float((got - want).norm() / want.norm()) <= 4 * own + 8 * ref.U + (2.0 ** -25 * 3.45 ** 5 if scale < 1 else 0.0)
     assert float(ops.orthogonalize(torch.zeros(1, m, n, device="cuda")).abs().max()) == 0
+
+
+@pytest.mark.parametrize("m,n", [(48, 72), (200, 144)])
+def test_result_over_the_input_through_another_tensors_storage(m, n):
+    # out's memory is the input's, shifted by one matrix, though their storages are not the same object or address
+    g = _matrix(4, m, n, torch.float32)
+    want = ops.orthogonalize(g[:3].cuda())
+    buf = g.cuda()
+    out = torch.from_dlpack(buf[1:])
+    assert out.untyped_storage().data_ptr() != buf.untyped_storage().data_ptr() and out.data_ptr() == buf[1].data_ptr()
+    assert torch.equal(ops.orthogonalize(buf[:3], out=out), want)
+    buf = g.cuda()
+    apart = ops.orthogonalize(buf[:2], out=buf[2:])  # one buffer, nothing shared
+    assert torch.equal(apart, want[:2]) and torch.equal(buf[:2], g[:2].cuda())
