@@ -223,6 +223,8 @@ def _differentiated(*tensors) -> bool:
     forward-mode form -- a dual number's tangent."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return True
+    if forward_ad._current_level < 0:  # (no dual numbers anywhere: a look at each tensor would cost as much as a small launch)
+        return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
