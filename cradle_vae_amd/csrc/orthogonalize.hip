@@ -7,10 +7,11 @@
 // times 2^12, which puts the lo plane of an entry of size 2^-6 (a 4096-wide matrix) well above fp16's subnormals and keeps
 // |X|, |S| = |X|^2 and |B| below 15.9 (checked for the coefficients by the caller) below its largest number.  fp32 results at three products of a rate
 // 16 times the fp32 matrix instruction's.  fp16 tensors take the same path: one plane's error would show in their last bits.
-// bf16 tensors multiply with the hi plane alone in all but the last two steps (X itself, and a X, keep both): early on the
-// singular values are small and so is everything (b S + c S S) X adds, so its 11-bit error barely reaches the result -- in an
-// emulation over full-rank, spiked, decaying and low-rank matrices the error after the final rounding is 1.00 to 1.22 times
-// that of the rounding alone, against up to 1.57 with one plane throughout (tests: 1.3).
+// bf16 tensors multiply with the hi plane alone in the first two steps of five (one_plane; X itself, and a X, keep both): of many
+// singular values all are small then, and so is everything (b S + c S S) X adds.  In an emulation over full-rank, orthogonal,
+// spiked, decaying and low-rank matrices (tests/test_operator_precision_cpu.py) the error after the final rounding is 1.00 to 1.06
+// times that of the rounding alone; with a third step of one plane it is up to 1.9, with few singular values up to 3.9 and
+// over 12 steps, all but two of them so, 28.
 // S and B are symmetric: only the tiles on and below the diagonal are computed, the epilogue stores them twice.
 // The norm is accumulated in fp64 (squares of fp32 gradients leave fp32's range).
 // Measured, five steps: 4096 x 8192 in bf16 4.33 ms (two-plane steps at 1040 TFLOP/s, one-plane steps at 815: the epilogue that reads
@@ -600,6 +601,12 @@ Layout layout_of(int64_t batch, int64_t m, int64_t n) {  // m <= n
   return l;
 }
 
+// Steps of a bf16 update whose products take X, S and B as one plane: early ones, three or more before the end (what a step gets
+// wrong is taken on by the next ones with slopes of up to 3.9, so not in long iterations either), of matrices with many singular
+// values (m: the smaller side).  4096 x 8192, five steps: two planes throughout 6.61 ms, this rule 5.13, one plane in a
+// third step 4.38; 2 x 513 x 1001: 193, 174 and 165 us.
+bool one_plane(int k, int m, int steps) { return k < 2 && k + 3 < steps && steps <= 8 && m >= 128; }
+
 int check_sizes(const char* what, int batch, int m, int n) {
   CRADLE_CHECK_ARG(batch >= 1 && batch <= 65535 && m >= 1 && n >= 1 && m <= (1 << 17) && n <= (1 << 17),
                    "%s: batch=%d m=%d n=%d (1 <= batch <= 65535, sides <= 2^17)", what, batch, m, n);
@@ -662,7 +669,7 @@ int cradle_orthogonalize(const void* g, int64_t ld_g, int64_t batch_stride_g, vo
                  sm, bm, l.s_plane, l.s_batch, M, N, l.lds, batch, b, c, partial, l.cs, l.cb, l.cx};
     const StepEpi epi{a, 1.f / kScale, x, x_next, l.x_plane, l.x_batch, l.ldx, k + 1 == steps ? out : nullptr, ld_out, batch_stride_out,
                       dtype, (int)flip, vec_out};
-    if (dtype == CRADLE_BF16 && k + 2 < steps) step<1>(t, epi, s);
+    if (dtype == CRADLE_BF16 && one_plane(k, M, steps)) step<1>(t, epi, s);
     else step<2>(t, epi, s);
     u16* next = x_next;
     x_next = x;

@@ -38,13 +38,14 @@ def test_fp32_block_beside_its_norm(M, K, F, O, act):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n", [(40, 56), (128, 128), (150, 420), (320, 200), (300, 1100), (513, 1001), (1500, 400)])
-def test_orthogonalised_update_beside_its_rounding(m, n, dtype):
+@pytest.mark.parametrize("m,n,steps", [(40, 56, 5), (128, 128, 5), (150, 420, 5), (320, 200, 5), (300, 1100, 5), (513, 1001, 5), (1500, 400, 5),
+                                       (769, 4, 5), (400, 32, 5), (5, 700, 5), (320, 900, 5), (140, 140, 4), (256, 256, 8), (320, 200, 12)])
+def test_orthogonalised_update_beside_its_rounding(m, n, steps, dtype):
     for kind, g in orth_matrices(m, n, dtype):
         g = g.cuda()
-        want = ref.orthogonalize(g, 5, ops.NS_COEFFS)
-        plain = ref.orthogonalize(g.float(), 5, ops.NS_COEFFS, dtype=torch.float32).double()
+        want = ref.orthogonalize(g, steps, ops.NS_COEFFS)
+        plain = ref.orthogonalize(g.float(), steps, ops.NS_COEFFS, dtype=torch.float32).double()
         own = float((plain - want).norm() / want.norm())
-        err = float((ops.orthogonalize(g).double() - want).norm() / want.norm())
+        err = float((ops.orthogonalize(g, steps=steps).double() - want).norm() / want.norm())
         limit = orth_limit(g, want, own)
         assert err <= limit, (kind, err, limit, own)
