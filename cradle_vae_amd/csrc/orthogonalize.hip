@@ -33,6 +33,20 @@ struct Tensor {
   int dtype, rows, cols;
 };
 
+// v -> v kScale / (|G|_F + eps), from the sum of squares.  The norm and its reciprocal can lie beyond fp32, so the divisor's power
+// of two goes first (exactly) and what is left of it, near one, second.
+struct Scale {
+  float two, rest;
+  __device__ __forceinline__ Scale(double sumsq, float eps) {
+    const double d = sqrt(sumsq) + (double)eps;
+    int e = (int)(__double2hiint(d) >> 20 & 0x7ff) - 1023;
+    e = e < -126 ? -126 : e > 149 ? 149 : e;
+    two = ldexpf(1.f, -e);
+    rest = kScale / (float)ldexp(d, -e);
+  }
+  __device__ __forceinline__ float operator()(float v) const { return v * two * rest; }
+};
+
 // partial sums of squares, (batch, gridDim.x) doubles: a wave takes every 4 gridDim.x-th row, 16 bytes per lane where rows allow
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void sumsq_kernel(const Tensor g, double* __restrict__ part) {
@@ -98,11 +112,11 @@ __global__ __launch_bounds__(256) void pack_kernel(const Tensor g, const double*
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   s = (red[0] + red[1]) + (red[2] + red[3]);
-  const double scale = kScale / (sqrt(s) + (double)eps);  // (in fp64: the norm or its reciprocal can lie beyond fp32)
+  const Scale scale(s, eps);
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int r = k * 4 + threadIdx.x / 64;
-    tile[r][c] = g0 + r < g.rows && g1 + c < g.cols ? (float)(v[k] * scale) : 0.f;
+    tile[r][c] = g0 + r < g.rows && g1 + c < g.cols ? scale(v[k]) : 0.f;
   }
   __syncthreads();
   u16* out = x + (int64_t)blockIdx.z * batch;
@@ -402,14 +416,14 @@ __global__ __launch_bounds__(kSmallThreads, 1) void small_kernel(const Tensor g,
   s = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) s += red[w];
-  const double scale = kScale / (sqrt(s) + (double)eps);  // (in fp64: the norm or its reciprocal can lie beyond fp32)
+  const Scale scale(s, eps);
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
     const int t = i * kSmallThreads + threadIdx.x;
     const int r = flip ? t % MP : t / (NP / 4), c0 = (flip ? t / MP : t % (NP / 4)) * 4;
     f32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = (float)(x[i][e] * scale);
+    for (int e = 0; e < 4; ++e) w[e] = scale(x[i][e]);
     store_planes<F16, 2>(small_at<NP>(X, r, c0), (int64_t)XP * 8, w);
   }
   __syncthreads();
