@@ -653,7 +653,8 @@ def gated_mlp_bwd(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: 
     _same_place(what, x, dy=dy, saved_gu=saved[0], saved_h=saved[1])
     lib, hb = hip.load(), ctypes.c_int64()
     gb = lib.cradle_gated_mlp_saved_bytes(M, d.width, F, O, d.dtype, ctypes.byref(hb))
-    if saved[0].numel() * 4 != gb or saved[1].numel() * 2 != hb.value:
+    if any(t.dtype is not dt or t.numel() * dt.itemsize != nbytes or not t.is_contiguous()
+           for t, dt, nbytes in zip(saved, (torch.float32, torch.int16), (gb, hb.value))):
         raise hip.CradleHipError(f"{what}: the saved buffers do not belong to a block of these sizes")
     new = x.new_empty if M else x.new_zeros
     dx = x.new_empty(x.shape) if need[0] else None

@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from cradle_vae_amd import functional as F_hip
-from cradle_vae_amd import ops
+from cradle_vae_amd import hip, ops
 from cradle_vae_amd.mlp import GaussianLikelihoodResidualMLP
 from cradle_vae_amd.optim import Muon
 from tests import operator_reference as ref
@@ -61,3 +61,16 @@ def test_hidden_matrices_of_every_type(dtype):
         off = 3 * 2e-5 * 0.02 * 0.2 * p.numel() ** 0.5 * 2 + 8 * ref.U * float(want[i].norm())
         off += 3 * ref.HALF[dtype] * float(want[i].norm()) * 1.1
         assert p.dtype == dtype and float((p.detach().double().cpu() - want[i]).norm()) <= off
+
+
+def test_saved_buffers_that_are_not_what_the_forward_pass_made():
+    p = {k: v.to(DEV) for k, v in _params().items()}
+    x, w_in, w_out, dy = p["x"], p["w_in"], p["w_out"], p["dy"]
+    _, (gu, h) = ops.gated_mlp(x, w_in, w_out, save=True)
+    want = ops.gated_mlp_bwd(dy, x, w_in, w_out, (gu, h))
+    # the right count of numbers in too small a memory, or of another type
+    for bad in ((gu[:1].expand(gu.shape), h), (gu, h[:1].expand(h.shape)), (gu.half(), h), (gu.int(), h), (gu, h.char()),
+                (torch.stack([gu, gu], 1)[:, 0], h), (gu[:-1], h), (gu, h[:-1]), (gu.cpu(), h)):
+        with pytest.raises(hip.CradleHipError):
+            ops.gated_mlp_bwd(dy, x, w_in, w_out, bad)
+    assert all(torch.equal(a, b) for a, b in zip(want[:3], ops.gated_mlp_bwd(dy, x, w_in, w_out, (gu, h))[:3]))
