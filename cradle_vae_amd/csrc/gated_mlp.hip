@@ -180,6 +180,7 @@ int cradle_gated_mlp_fwd(const cradle_gated_mlp_desc* d, cradle_stream_t s) {
   if (rc != CRADLE_OK) return rc;
   if (d->rows == 0) return CRADLE_OK;
   CRADLE_CHECK_ARG(d->x && d->w_in && d->w_out && d->y, "gated_mlp_fwd: null pointer");
+  CRADLE_CHECK_ARG(((uintptr_t)d->saved_gu & 15) == 0 && ((uintptr_t)d->saved_h & 15) == 0, "gated_mlp_fwd: saved buffers must be 16-byte aligned");
   CRADLE_CHECK_ARG(d->ld_y >= d->out_width && (!d->residual || d->ld_residual >= d->out_width), "gated_mlp_fwd: leading dimension below the row length");
   const int64_t need = cradle_gated_mlp_workspace_bytes(d, 0);
   CRADLE_CHECK_ARG(need == 0 || (d->workspace && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15) == 0),

@@ -443,7 +443,7 @@ int cradle_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
 /* Gated feed-forward block: [g | u] = x W_in^T + b_in, h = act(g) * u, y = h W_out^T + b_out (+ residual).
  * x (rows, width); w_in (2 hidden, width): the gate's rows, then the up projection's; w_out (out_width, hidden); b_in
  * (2 hidden), b_out (out_width) or NULL; residual (rows, out_width) or NULL; y (rows, out_width).  act: 0 silu, 1 gelu (erf).
- * Training: saved_gu and saved_h (cradle_gated_mlp_saved_bytes) receive what the backward pass reads; NULL for inference.
+ * Training: saved_gu and saved_h (cradle_gated_mlp_saved_bytes) receive what the backward pass reads, 16-byte aligned; NULL for inference.
  * cradle_gated_mlp_bwd: from dy (rows, out_width) and the saved buffers, dx (rows, width; NULL = not needed), dw_in, dw_out
  * (contiguous, NULL = not needed), db_in, db_out (NULL = not needed).  The residual's gradient is dy.
  * h and [dg | du] are rounded to the tensors' type where they enter a matrix product (fp32: to 24 bits; 16-bit types of small
