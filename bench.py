@@ -86,11 +86,11 @@ def k1_pmc_traffic(G, N, P):
 
 def profiled_avg_us(substr):
     """Average duration of a kernel in the committed rocprofv3 --kernel-trace --stats summary of this command
-    (profiles/r03_bench_kernel_stats.csv), for the reader's comparison with the live figure: the HIP events of the live
+    (profiles/scalar_fp32_bench_kernel_stats.csv), for the reader's comparison with the live figure: the HIP events of the live
     bracket add their own ~3 us of marker packets between dependent kernels.  None when the file is not there."""
     import csv
 
-    path = os.path.join(ROOT, "profiles", "r03_bench_kernel_stats.csv")
+    path = os.path.join(ROOT, "profiles", "scalar_fp32_bench_kernel_stats.csv")
     try:
         with open(path) as f:
             rows = [r for r in csv.DictReader(f) if substr in r.get("Name", "")]

@@ -14,9 +14,10 @@
 // The saved pre-activations stay fp32 (rounded to bf16 they would put two more roundings into every gradient).
 // A handful of rows (inference of single cells) take kernels that read the weights once, coalesced, with fp32 arithmetic.
 //
-// Measured, forward and backward: 8192 rows, 4096 x 10240 in bf16 5.2 ms, 1190 TFLOP/s (library products of these sizes: 1290 to 1560),
-// bound by the matrix cores and the epilogues that a 256 x 256 tile, alone on its CU, does not hide; 1537 rows, 1000 x 2731 in fp16
-// 193 us and 2560 rows, 400 x 800 in fp32 161 us, bound by the loads' latency over sums of 13 to 30 K tiles.
+// Measured on two cards, forward and backward: 8192 rows, 4096 x 10240 in bf16 5.2 and 5.3 ms, 1160 to 1190 TFLOP/s (library products
+// of these sizes: 1290 to 1560), bound by the matrix cores and the epilogues that a 256 x 256 tile, alone on its CU, does not
+// hide; 1537 rows, 1000 x 2731 in fp16 195 and 199 us and 2560 rows, 400 x 800 in fp32 161 and 168 us, bound by the loads' latency
+// over sums of 13 to 30 K tiles.
 #pragma once
 #include <type_traits>
 

@@ -14,9 +14,9 @@
 // over 12 steps, all but two of them so, 28.
 // S and B are symmetric: only the tiles on and below the diagonal are computed, the epilogue stores them twice.
 // The norm is accumulated in fp64 (squares of fp32 gradients leave fp32's range).
-// Measured, five steps: 4096 x 8192 in bf16 4.33 ms (two-plane steps at 1040 TFLOP/s, one-plane steps at 815: the epilogue that reads
-// and writes both planes of X is not hidden); 5000 x 400 in fp32 209 us, 2 x 513 x 1001 in fp16 192 us: chains of 17 to 22 launches
-// of 5 to 16 us.
+// Measured, five steps: 4096 x 8192 in bf16 5.14 and 5.28 ms on two cards (two-plane steps at 1060 TFLOP/s, one-plane steps at 830:
+// the epilogue that reads and writes both planes of X is not hidden); 5000 x 400 in fp32 209 us, 2 x 513 x 1001 in fp16 192 us: chains
+// of 22 and 17 launches of 4 to 15 us.
 #include "mm16.h"
 
 namespace cradle {
