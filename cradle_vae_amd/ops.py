@@ -712,7 +712,9 @@ def _ns_holds(coeffs, steps: int) -> bool:
 def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of each matrix of ``g`` (..., m, n), fp32 / bf16 / fp16: X = G / (|G|_F + eps), then
     ``steps`` times X <- a X + (b S + c S S) X with S = X X^T on the smaller side (``cradle_orthogonalize``); every singular value s
-    goes through a s + b s^3 + c s^5.  fp32 accuracy inside, one rounding to g's type.  ``out`` may be ``g``.  Coefficients
+    goes through a s + b s^3 + c s^5.  fp32 accuracy inside, one rounding to g's type (bf16 with a smaller side from 128 on:
+    the first two of five to eight steps, of four the first, multiply 11 bits, which adds at most a tenth to the error of that
+    rounding).  ``out`` may be ``g``.  Coefficients
     whose iteration from a start in [0, 1] reaches 7.95, or brings 3.98 (S: 15.9) into another step, are refused (the
     products hold X, S and b S + c S S times 2^12 in fp16 planes)."""
     what = "orthogonalize"

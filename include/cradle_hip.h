@@ -481,7 +481,8 @@ int cradle_gated_mlp_bwd(const cradle_gated_mlp_desc* desc, cradle_stream_t stre
 /* ---- Orthogonalised update of a weight matrix (an optimiser beside K10; no counterpart in the reference) -------------------
  * For each of `batch` matrices G (m, n): X = G / (|G|_F + eps); `steps` times S = X X^T, X <- a X + (b S + c S S) X (on the
  * smaller side); out = X.  g, out: CRADLE_F32 / BF16 / F16, rows contiguous, leading dimensions and batch strides in elements.
- * fp32 accuracy throughout, one rounding to the output's type.  The polynomial s -> a s + b s^3 + c s^5, iterated from [0, 1],
+ * fp32 accuracy throughout, one rounding to the output's type (bf16, smaller side >= 128: early steps multiply 11 bits, which adds
+ * at most a tenth to the error of that rounding).  The polynomial s -> a s + b s^3 + c s^5, iterated from [0, 1],
  * has to stay below 7.95 in magnitude together with b s^2 + c s^4, and below 3.98 wherever another step follows (the caller
  * checks its coefficients; X, S -- whose eigenvalues are s^2 -- and b S + c S S are held times 2^12 in fp16 planes and overflow
  * to infinity from 16 on).  out may be g itself, not overlap it otherwise.  workspace: cradle_orthogonalize_workspace_bytes bytes, 16-byte aligned. */
